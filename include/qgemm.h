@@ -168,6 +168,53 @@ typedef enum qgemm_quant_mode {
 int qgemm_quantize(int in_dtype, int out_dtype, int mode, const void *x, size_t ld, size_t rows, size_t cols, void *q,
                    size_t ldq, float *scales, size_t scale_rs, size_t scale_cs, void *stream);
 
+/* ---- Training around the products (no counterpart in the reference): layer norm, activations kept in 8 bits for the backward
+ * pass, and the gradients computed from them.
+ *
+ * An activation in 8 bits ("kept", "codes") is rows x cols bytes (I8 or F8E4M3) and one float for 128 columns of a row,
+ * scales[row * ceil(cols / 128) + col / 128], the arrangement of QGEMM_QUANT_BLOCK_1x128 with K-contiguous scales; it stands for q * scale.
+ * What the entries below write has powers of two as scales: s is the smallest (2^-126 at the least) with max|v| <= 127 s (448 s), 1
+ * for a block of zeros, q = rne(v / s); at the top of the type's range codes stop where q * s would be infinite.  q * s is then exact in
+ * bf16 (and in fp16 down to its smallest numbers).  A block with an infinity or NaN gets s = NaN and reads as NaN throughout.  What the
+ * entries below read may have any scales, those of qgemm_quantize among them.
+ *
+ * Types are F32, BF16 or F16 unless said otherwise; leading dimensions count elements.  Zero rows are no error: gradients
+ * of parameters are then zeros.  All sums are fp32, in an order that is the same from run to run. */
+
+/* y = xhat * weight + bias, xhat = (x - mean) * rstd, for every row: mean = sum x / cols, rstd = 1 / sqrt(sum (x - mean)^2 / cols + eps).
+ *   weight, bias  cols elements of param_dtype each; weight NULL: y = xhat, bias NULL: none (a bias needs a weight)
+ *   mean, rstd    rows floats each, for the backward pass; NULL where nobody wants them
+ *   q, scales     xhat in 8 bits, of q_dtype, as qgemm_layer_norm_backward and qgemm_weight_gradient read it; both NULL: not written */
+int qgemm_layer_norm(int x_dtype, int y_dtype, int param_dtype, int q_dtype, const void *x, size_t ldx, const void *weight, const void *bias,
+                     float eps, void *y, size_t ldy, float *mean, float *rstd, void *q, size_t ldq, float *scales, size_t rows,
+                     size_t cols, void *stream);
+
+/* Backward pass of qgemm_layer_norm: with g = dy * weight
+ *   dx = rstd * (g - sum(g) / cols - xhat * sum(g * xhat) / cols), dweight = sum over rows of dy * xhat, dbias = sum over rows of dy
+ *   x        the norm's input (mean is needed then), or xhat in 8 bits: x_dtype I8 / F8E4M3 with its scales (mean is ignored)
+ *   dweight, dbias  cols elements of param_dtype each, overwritten; NULL where nobody wants them.  Partial sums go through the
+ *            library workspace */
+int qgemm_layer_norm_backward(int dy_dtype, int x_dtype, int dx_dtype, int param_dtype, const void *dy, size_t lddy, const void *x, size_t ldx,
+                              const float *scales, const float *mean, const float *rstd, const void *weight, void *dx, size_t lddx,
+                              void *dweight, void *dbias, size_t rows, size_t cols, void *stream);
+
+/* An activation into 8 bits, and back (x = q * scale, rounded once where x_dtype has fewer bits). */
+int qgemm_checkpoint(int x_dtype, int q_dtype, const void *x, size_t ldx, size_t rows, size_t cols, void *q, size_t ldq, float *scales,
+                     void *stream);
+int qgemm_restore(int q_dtype, int x_dtype, const void *q, size_t ldq, const float *scales, size_t rows, size_t cols, void *x, size_t ldx,
+                  void *stream);
+
+/* Gradients of a linear layer z = v W^T + c out of its input v in 8 bits:
+ *   dw[n x cols] = dy^T v and db[n] = sum over rows of dy
+ *   dy       rows x n, BF16 or F16: v is widened to that type in front of the matrix cores (exact where scales are powers of two;
+ *            F16: beyond 65504 infinite)
+ *   weight, bias  cols elements of param_dtype each, or NULL: q holds a layer norm's xhat and v = xhat * weight + bias is meant
+ *   dw       of dw_dtype, overwritten; fp32 accumulation.  Few tiles of it split the rows between workgroups through the library workspace
+ *   db       n floats, or NULL */
+int qgemm_weight_gradient(int dy_dtype, int q_dtype, int dw_dtype, int param_dtype, const void *dy, size_t lddy, const void *q, size_t ldq,
+                          const float *scales, const void *weight, const void *bias, void *dw, size_t lddw, float *db, size_t rows,
+                          size_t n, size_t cols, void *stream);
+
 /* Tile raster used by the GEMM kernels: linear workgroup id -> (tile_m, tile_n).
  * Replaces the GROUP_SIZE_M swizzle of src/gemm/sm89_gemm_kernel_v3.cu:169-183
  * (and fixes its clamp), composed with the 8-XCD remap the reference only names

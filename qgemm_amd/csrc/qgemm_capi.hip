@@ -16,6 +16,7 @@
 #include "gemm_any.cuh"
 #include "quant_kernels.cuh"
 #include "selftest.cuh"
+#include "training.h"
 #include "variants.h"
 
 using namespace qgemm;
@@ -1799,6 +1800,30 @@ int quantize_t(int mode, QuantArgs &a, hipStream_t stream) {
     return e == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
 }
 
+bool is_float_type(int dt) { return dt == QGEMM_DT_F32 || dt == QGEMM_DT_BF16 || dt == QGEMM_DT_F16; }
+bool is_code_type(int dt) { return dt == QGEMM_DT_I8 || dt == QGEMM_DT_F8E4M3; }
+uint32_t blocks_of(size_t cols) { return (uint32_t)((cols + kScaleBlock - 1) / kScaleBlock); }
+
+// Body of qgemm_checkpoint (`encode`) and qgemm_restore
+int keep_entry(bool encode, int in_dt, int out_dt, const void *in, size_t ld_in, void *out, size_t ld_out, float *scales, size_t rows, size_t cols,
+               void *stream) {
+    if (rows >= ((size_t)1 << 31) || cols >= ((size_t)1 << 31)) return QGEMM_ERR_TOO_LARGE;
+    if (rows == 0 || cols == 0) return QGEMM_OK;
+    if (!in || !out || !scales || ld_in < cols || ld_out < cols) return QGEMM_ERR_INVALID_ARG;
+    std::lock_guard<std::mutex> lock(g_ctx.mu);
+    const int st = ensure_init_locked();
+    if (st != QGEMM_OK) return st;
+    KeepArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.in = in, a.out = out, a.scales = scales;
+    a.ld_in = ld_in, a.ld_out = ld_out;
+    a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.kb = blocks_of(cols);
+    a.in_dt = in_dt, a.out_dt = out_dt;
+    g_ctx.last_config = encode ? "checkpoint" : "restore";
+    const hipError_t e = encode ? launch_checkpoint(a, (hipStream_t)stream) : launch_restore(a, (hipStream_t)stream);
+    return e == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+}
+
 }  // namespace
 
 // ===========================================================================
@@ -2064,6 +2089,108 @@ QGEMM_EXPORT int qgemm_transpose(int elem_bytes, const void *in, void *out, size
     int st = ensure_init_locked();
     if (st != QGEMM_OK) return st;
     return launch_transpose(elem_bytes, in, out, M, N, (hipStream_t)stream);
+}
+
+QGEMM_EXPORT int qgemm_layer_norm(int x_dtype, int y_dtype, int param_dtype, int q_dtype, const void *x, size_t ldx, const void *weight,
+                                  const void *bias, float eps, void *y, size_t ldy, float *mean, float *rstd, void *q, size_t ldq,
+                                  float *scales, size_t rows, size_t cols, void *stream_) {
+    if (!is_float_type(x_dtype) || !is_float_type(y_dtype)) return QGEMM_ERR_UNSUPPORTED;
+    if (weight && !is_float_type(param_dtype)) return QGEMM_ERR_UNSUPPORTED;
+    if (q && !is_code_type(q_dtype)) return QGEMM_ERR_UNSUPPORTED;
+    if (cols == 0 || !(eps >= 0.0f) || (bias && !weight) || (!q) != (!scales)) return QGEMM_ERR_INVALID_ARG;
+    if (rows >= ((size_t)1 << 31) || cols >= ((size_t)1 << 31)) return QGEMM_ERR_TOO_LARGE;
+    if (rows == 0) return QGEMM_OK;
+    if (!x || !y || ldx < cols || ldy < cols || (q && ldq < cols)) return QGEMM_ERR_INVALID_ARG;
+    std::lock_guard<std::mutex> lock(g_ctx.mu);
+    const int st = ensure_init_locked();
+    if (st != QGEMM_OK) return st;
+    NormArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.x = x, a.weight = weight, a.bias = bias;
+    a.y = y, a.q = q;
+    a.mean = mean, a.rstd = rstd, a.scales = scales;
+    a.ldx = ldx, a.ldy = ldy, a.ldq = ldq;
+    a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.kb = blocks_of(cols);
+    a.eps = eps;
+    a.x_dt = x_dtype, a.y_dt = y_dtype, a.param_dt = param_dtype, a.q_dt = q_dtype;
+    g_ctx.last_config = "layer_norm";
+    return launch_layer_norm(a, g_ctx.num_cus, (hipStream_t)stream_) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+}
+
+QGEMM_EXPORT int qgemm_layer_norm_backward(int dy_dtype, int x_dtype, int dx_dtype, int param_dtype, const void *dy, size_t lddy, const void *x,
+                                           size_t ldx, const float *scales, const float *mean, const float *rstd, const void *weight,
+                                           void *dx, size_t lddx, void *dweight, void *dbias, size_t rows, size_t cols, void *stream_) {
+    const bool codes = is_code_type(x_dtype);
+    if (!is_float_type(dy_dtype) || !is_float_type(dx_dtype) || (!is_float_type(x_dtype) && !codes)) return QGEMM_ERR_UNSUPPORTED;
+    if ((weight || dweight || dbias) && !is_float_type(param_dtype)) return QGEMM_ERR_UNSUPPORTED;
+    if (cols == 0) return QGEMM_ERR_INVALID_ARG;
+    if (rows >= ((size_t)1 << 31) || cols >= ((size_t)1 << 31)) return QGEMM_ERR_TOO_LARGE;
+    if (rows && (!dy || !x || !dx || !rstd || (codes ? !scales : !mean) || lddy < cols || ldx < cols || lddx < cols)) return QGEMM_ERR_INVALID_ARG;
+    if (rows == 0 && !dweight && !dbias) return QGEMM_OK;
+    hipStream_t stream = (hipStream_t)stream_;
+    std::lock_guard<std::mutex> lock(g_ctx.mu);
+    int st = ensure_init_locked();
+    if (st != QGEMM_OK) return st;
+    WorkspaceUse ws_use(stream);
+    NormBackwardArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.dy = dy, a.x = x, a.weight = weight;
+    a.scales = scales, a.mean = mean, a.rstd = rstd;
+    a.dx = dx, a.dweight = dweight, a.dbias = dbias;
+    a.lddy = lddy, a.ldx = ldx, a.lddx = lddx;
+    a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.kb = blocks_of(cols);
+    a.dy_dt = dy_dtype, a.x_dt = x_dtype, a.dx_dt = dx_dtype, a.param_dt = param_dtype;
+    a.groups = norm_backward_groups(a, g_ctx.num_cus);
+    if (a.groups) {
+        void *ws = nullptr;
+        st = ensure_workspace_locked(norm_partial_bytes(a.groups, a.cols), stream, &ws);
+        if (st != QGEMM_OK) return st;
+        a.partial = (float *)ws;
+    }
+    g_ctx.last_config = "layer_norm_backward";
+    return launch_layer_norm_backward(a, g_ctx.num_cus, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+}
+
+QGEMM_EXPORT int qgemm_checkpoint(int x_dtype, int q_dtype, const void *x, size_t ldx, size_t rows, size_t cols, void *q, size_t ldq, float *scales,
+                                  void *stream) {
+    if (!is_float_type(x_dtype) || !is_code_type(q_dtype)) return QGEMM_ERR_UNSUPPORTED;
+    return keep_entry(true, x_dtype, q_dtype, x, ldx, q, ldq, scales, rows, cols, stream);
+}
+
+QGEMM_EXPORT int qgemm_restore(int q_dtype, int x_dtype, const void *q, size_t ldq, const float *scales, size_t rows, size_t cols, void *x, size_t ldx,
+                               void *stream) {
+    if (!is_float_type(x_dtype) || !is_code_type(q_dtype)) return QGEMM_ERR_UNSUPPORTED;
+    return keep_entry(false, q_dtype, x_dtype, q, ldq, x, ldx, const_cast<float *>(scales), rows, cols, stream);
+}
+
+QGEMM_EXPORT int qgemm_weight_gradient(int dy_dtype, int q_dtype, int dw_dtype, int param_dtype, const void *dy, size_t lddy, const void *q, size_t ldq,
+                                       const float *scales, const void *weight, const void *bias, void *dw, size_t lddw, float *db, size_t rows,
+                                       size_t n, size_t cols, void *stream_) {
+    if ((dy_dtype != QGEMM_DT_BF16 && dy_dtype != QGEMM_DT_F16) || !is_code_type(q_dtype) || !is_float_type(dw_dtype)) return QGEMM_ERR_UNSUPPORTED;
+    if (weight && !is_float_type(param_dtype)) return QGEMM_ERR_UNSUPPORTED;
+    if (cols == 0 || (bias && !weight)) return QGEMM_ERR_INVALID_ARG;
+    if (rows >= ((size_t)1 << 31) || n >= ((size_t)1 << 31) || cols >= ((size_t)1 << 31)) return QGEMM_ERR_TOO_LARGE;
+    if (n == 0) return QGEMM_OK;
+    if (!dw || lddw < cols || (rows && (!dy || !q || !scales || lddy < n || ldq < cols))) return QGEMM_ERR_INVALID_ARG;
+    hipStream_t stream = (hipStream_t)stream_;
+    std::lock_guard<std::mutex> lock(g_ctx.mu);
+    int st = ensure_init_locked();
+    if (st != QGEMM_OK) return st;
+    WorkspaceUse ws_use(stream);
+    WeightGradArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.dy = dy, a.q = q, a.weight = weight, a.bias = bias;
+    a.scales = scales;
+    a.dw = dw, a.db = db;
+    a.lddy = lddy, a.ldq = ldq, a.lddw = lddw;
+    a.rows = (uint32_t)rows, a.n = (uint32_t)n, a.cols = (uint32_t)cols, a.kb = blocks_of(cols);
+    a.dy_dt = dy_dtype, a.q_dt = q_dtype, a.param_dt = param_dtype, a.dw_dt = dw_dtype;
+    if (const size_t room = weight_grad_room(a, g_ctx.num_cus)) {
+        st = ensure_workspace_locked(room, stream, &a.room);
+        if (st != QGEMM_OK) return st;
+    }
+    g_ctx.last_config = "weight_gradient";
+    return launch_weight_grad(a, g_ctx.num_cus, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
 }
 
 QGEMM_EXPORT int qgemm_gemm(int in_dtype, int out_dtype, int layout_b, const void *A, size_t ldA, const void *B, size_t ldB,

@@ -180,6 +180,156 @@ std::tuple<int, at::Tensor, at::Tensor> ops_quantize(const at::Tensor &x, at::Sc
     return {st, q, scales};
 }
 
+// ---- layer norm, activations in 8 bits, weight gradients
+// t as rows of its last dimension, evenly spaced `ld` elements apart, the elements of a row side by side; false where it is not
+bool rows_of(const at::Tensor &t, int64_t &rows, int64_t &cols, int64_t &ld) {
+    const int64_t d = t.dim();
+    if (d < 1) return false;
+    rows = 1;
+    cols = t.size(d - 1);
+    if (cols < 1 || (cols > 1 && t.stride(d - 1) != 1)) return false;
+    int64_t step = 0;                                      // from a row to the next
+    for (int64_t i = d - 2; i >= 0; --i) {
+        const int64_t n = t.size(i);
+        if (n == 1) continue;
+        if (rows == 1) step = t.stride(i);
+        else if (t.stride(i) != rows * step && n > 0) return false;
+        rows *= n;
+        if (rows == 0) break;
+    }
+    for (int64_t i = 0; i + 1 < d; ++i)
+        if (t.size(i) == 0) rows = 0;
+    ld = rows > 1 ? step : cols;
+    return ld >= cols;
+}
+bool float_vector(const at::Tensor &t, int64_t n) { return t.is_cuda() && t.scalar_type() == at::kFloat && t.numel() == n && t.is_contiguous(); }
+bool float_dtype(int dt) { return dt == QGEMM_DT_F32 || dt == QGEMM_DT_BF16 || dt == QGEMM_DT_F16; }
+int code_dtype(at::ScalarType t) { return t == at::kChar ? QGEMM_DT_I8 : t == at::kFloat8_e4m3fn ? QGEMM_DT_F8E4M3 : -1; }
+// a layer norm's parameters: one or both, of one type
+bool parameters_ok(const std::optional<at::Tensor> &weight, const std::optional<at::Tensor> &bias, int64_t cols, int &dt) {
+    dt = QGEMM_DT_F32;
+    if (!weight) return !bias;
+    dt = plain_dtype(*weight, false);
+    auto ok = [&](const at::Tensor &t) { return t.is_cuda() && t.numel() == cols && t.is_contiguous(); };
+    return float_dtype(dt) && ok(*weight) && (!bias || (ok(*bias) && bias->scalar_type() == weight->scalar_type()));
+}
+const void *data_or_null(const std::optional<at::Tensor> &t) { return t ? t->data_ptr() : nullptr; }
+at::DimVector with_last(const at::Tensor &t, int64_t last) {
+    at::DimVector v(t.sizes().begin(), t.sizes().end());
+    v.back() = last;
+    return v;
+}
+
+// (status, y, mean, rstd, q, scales)
+typedef std::tuple<int, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> NormOut;
+NormOut ops_layer_norm(const at::Tensor &x, const std::optional<at::Tensor> &weight, const std::optional<at::Tensor> &bias, double eps,
+                       std::optional<at::ScalarType> out, std::optional<at::ScalarType> keep) {
+    NormOut r;
+    std::get<0>(r) = kNotPlain;
+    int64_t rows, cols, ld;
+    int pdt;
+    if (!x.is_cuda() || !rows_of(x, rows, cols, ld) || !parameters_ok(weight, bias, cols, pdt)) return r;
+    const int xdt = plain_dtype(x, false), qdt = keep ? code_dtype(*keep) : 0;
+    if (!float_dtype(xdt) || qdt < 0) return r;
+    at::Tensor y = at::empty(x.sizes(), out ? x.options().dtype(*out) : x.options());
+    const int ydt = plain_dtype(y, false);
+    if (!float_dtype(ydt)) return r;
+    const auto f32 = x.options().dtype(at::kFloat);
+    const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
+    at::Tensor mean = at::empty(lead, f32), rstd = at::empty(lead, f32), q, scales;
+    if (keep) {
+        q = at::empty(x.sizes(), x.options().dtype(*keep));
+        scales = at::empty(with_last(x, (cols + 127) / 128), f32);
+    }
+    int st;
+    {
+        py::gil_scoped_release no_gil;
+        st = qgemm_layer_norm(xdt, ydt, pdt, qdt, x.data_ptr(), ld, data_or_null(weight), data_or_null(bias), (float)eps, y.data_ptr(), cols,
+                              (float *)mean.data_ptr(), (float *)rstd.data_ptr(), keep ? q.data_ptr() : nullptr, cols,
+                              keep ? (float *)scales.data_ptr() : nullptr, rows, cols, current_stream());
+    }
+    return {st, y, mean, rstd, q, scales};
+}
+
+// (status, dx, dweight, dbias)
+typedef std::tuple<int, at::Tensor, at::Tensor, at::Tensor> NormBackwardOut;
+NormBackwardOut ops_layer_norm_backward(const at::Tensor &dy, const at::Tensor &x, const std::optional<at::Tensor> &mean, const at::Tensor &rstd,
+                                        const std::optional<at::Tensor> &weight, const std::optional<at::Tensor> &scales, bool bias,
+                                        std::optional<at::ScalarType> out) {
+    NormBackwardOut r;
+    std::get<0>(r) = kNotPlain;
+    int64_t rows, cols, lddy, xrows, xcols, ldx;
+    int pdt;
+    if (!dy.is_cuda() || !x.is_cuda() || !rows_of(dy, rows, cols, lddy) || !rows_of(x, xrows, xcols, ldx) || xrows != rows || xcols != cols ||
+        !parameters_ok(weight, std::nullopt, cols, pdt) || !float_vector(rstd, rows))
+        return r;
+    const int codes = code_dtype(x.scalar_type()), xdt = codes >= 0 ? codes : plain_dtype(x, false), dydt = plain_dtype(dy, false);
+    if (!float_dtype(dydt) || (codes < 0 && !float_dtype(xdt))) return r;
+    if (codes >= 0 ? !scales || !float_vector(*scales, rows * ((cols + 127) / 128)) : !mean || scales || !float_vector(*mean, rows)) return r;
+    at::Tensor dx = at::empty(dy.sizes(), out ? dy.options().dtype(*out) : dy.options()), dw, db;
+    const int dxdt = plain_dtype(dx, false);
+    if (!float_dtype(dxdt)) return r;
+    if (weight) {
+        dw = at::empty_like(*weight);
+        if (bias) db = at::empty_like(*weight);
+    }
+    int st;
+    {
+        py::gil_scoped_release no_gil;
+        st = qgemm_layer_norm_backward(dydt, xdt, dxdt, pdt, dy.data_ptr(), lddy, x.data_ptr(), ldx, (const float *)data_or_null(scales),
+                                       (const float *)data_or_null(mean), (const float *)rstd.data_ptr(), data_or_null(weight), dx.data_ptr(), cols,
+                                       dw.defined() ? dw.data_ptr() : nullptr, db.defined() ? db.data_ptr() : nullptr, rows, cols, current_stream());
+    }
+    return {st, dx, dw, db};
+}
+
+// (status, q, scales)
+std::tuple<int, at::Tensor, at::Tensor> ops_checkpoint(const at::Tensor &x, at::ScalarType out) {
+    const std::tuple<int, at::Tensor, at::Tensor> not_plain{kNotPlain, at::Tensor(), at::Tensor()};
+    int64_t rows, cols, ld;
+    const int qdt = code_dtype(out);
+    if (!x.is_cuda() || qdt < 0 || !rows_of(x, rows, cols, ld)) return not_plain;
+    const int xdt = plain_dtype(x, false);
+    if (!float_dtype(xdt)) return not_plain;
+    at::Tensor q = at::empty(x.sizes(), x.options().dtype(out)), scales = at::empty(with_last(x, (cols + 127) / 128), x.options().dtype(at::kFloat));
+    py::gil_scoped_release no_gil;
+    return {qgemm_checkpoint(xdt, qdt, x.data_ptr(), ld, rows, cols, q.data_ptr(), cols, (float *)scales.data_ptr(), current_stream()), q, scales};
+}
+
+// (status, x)
+std::tuple<int, at::Tensor> ops_restore(const at::Tensor &q, const at::Tensor &scales, at::ScalarType out) {
+    int64_t rows, cols, ld;
+    const int qdt = code_dtype(q.scalar_type());
+    if (!q.is_cuda() || qdt < 0 || !rows_of(q, rows, cols, ld) || !float_vector(scales, rows * ((cols + 127) / 128))) return {kNotPlain, at::Tensor()};
+    at::Tensor x = at::empty(q.sizes(), q.options().dtype(out));
+    const int xdt = plain_dtype(x, false);
+    if (!float_dtype(xdt)) return {kNotPlain, at::Tensor()};
+    py::gil_scoped_release no_gil;
+    return {qgemm_restore(qdt, xdt, q.data_ptr(), ld, (const float *)scales.data_ptr(), rows, cols, x.data_ptr(), cols, current_stream()), x};
+}
+
+// (status, dw, db)
+std::tuple<int, at::Tensor, at::Tensor> ops_weight_gradient(const at::Tensor &dy, const at::Tensor &q, const at::Tensor &scales,
+                                                            const std::optional<at::Tensor> &weight, const std::optional<at::Tensor> &bias,
+                                                            at::ScalarType out) {
+    const std::tuple<int, at::Tensor, at::Tensor> not_plain{kNotPlain, at::Tensor(), at::Tensor()};
+    int64_t rows, n, lddy, qrows, cols, ldq;
+    int pdt;
+    const int qdt = code_dtype(q.scalar_type());
+    if (!dy.is_cuda() || !q.is_cuda() || qdt < 0 || !rows_of(dy, rows, n, lddy) || !rows_of(q, qrows, cols, ldq) || qrows != rows ||
+        !parameters_ok(weight, bias, cols, pdt) || !float_vector(scales, rows * ((cols + 127) / 128)))
+        return not_plain;
+    const int dydt = plain_dtype(dy, false);
+    if (dydt != QGEMM_DT_BF16 && dydt != QGEMM_DT_F16) return not_plain;
+    at::Tensor dw = at::empty({n, cols}, dy.options().dtype(out)), db = at::empty({n}, dy.options().dtype(at::kFloat));
+    const int dwdt = plain_dtype(dw, false);
+    if (!float_dtype(dwdt)) return not_plain;
+    py::gil_scoped_release no_gil;
+    return {qgemm_weight_gradient(dydt, qdt, dwdt, pdt, dy.data_ptr(), lddy, q.data_ptr(), ldq, (const float *)scales.data_ptr(), data_or_null(weight),
+                                  data_or_null(bias), dw.data_ptr(), cols, (float *)db.data_ptr(), rows, n, cols, current_stream()),
+            dw, db};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -192,4 +342,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("ops_scaled_gemm", &ops_scaled_gemm);
     m.def("ops_transpose", &ops_transpose);
     m.def("ops_quantize", &ops_quantize);
+    m.def("ops_layer_norm", &ops_layer_norm);
+    m.def("ops_layer_norm_backward", &ops_layer_norm_backward);
+    m.def("ops_checkpoint", &ops_checkpoint);
+    m.def("ops_restore", &ops_restore);
+    m.def("ops_weight_gradient", &ops_weight_gradient);
 }

@@ -44,6 +44,11 @@ SIGNATURES = {
     "qgemm_workspace_info": (_i, [C.POINTER(_vp), C.POINTER(_sz)]),
     "qgemm_transpose": (_i, [_i, _vp, _vp, _sz, _sz, _vp]),
     "qgemm_quantize": (_i, [_i, _i, _i, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _vp]),
+    "qgemm_layer_norm": (_i, [_i, _i, _i, _i, _vp, _sz, _vp, _vp, C.c_float, _vp, _sz, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _vp]),
+    "qgemm_layer_norm_backward": (_i, [_i, _i, _i, _i, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp]),
+    "qgemm_checkpoint": (_i, [_i, _i, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _vp]),
+    "qgemm_restore": (_i, [_i, _i, _vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp]),
+    "qgemm_weight_gradient": (_i, [_i, _i, _i, _i, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz, _vp]),
     "qgemm_tile_map": (_i, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint32),
                             C.POINTER(C.c_uint32)]),
     "qgemm_quantize_grid": (_i, [_i, _sz, _sz, C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint32)]),

@@ -6,6 +6,9 @@
   matrix_transpose(in, out)    src/transpose/transpose.cu:60-74
   gemm(...)                    GEMM_kernel_v*<In, Out> of include/gemm.h:25-66
   quantize(x, ...)             the Q_A / Q_B of README.md:1 (the reference has no quantiser)
+  layer_norm(x, ...), layer_norm_backward(dy, x, ...), checkpoint(x, ...), restore(q, scales, ...), weight_gradient(dy, q, scales, ...)
+                               training around the products: a layer norm, activations kept in 8 bits, the gradients computed
+                               from them (no counterpart in the reference)
 
 Tensors are torch CUDA(HIP) tensors; only their data pointers and the current
 stream cross the boundary."""
@@ -30,6 +33,8 @@ _TORCH_DT = {
 
 
 _native_module = None
+_NATIVE_ENTRIES = ("ops_gemm", "ops_scaled_gemm", "ops_transpose", "ops_quantize", "ops_layer_norm", "ops_layer_norm_backward", "ops_checkpoint",
+                   "ops_restore", "ops_weight_gradient")
 
 
 def _native():
@@ -44,7 +49,7 @@ def _native():
             load_library()                      # (its absence is an error, not a reason to go another way)
             try:
                 module = load_torch_extension()
-                missing = [f for f in ("ops_gemm", "ops_scaled_gemm", "ops_transpose", "ops_quantize") if not hasattr(module, f)]
+                missing = [f for f in _NATIVE_ENTRIES if not hasattr(module, f)]
                 if missing:
                     raise ImportError(f"{getattr(module, '__file__', 'qgemm_python')} has no {', '.join(missing)}: build it again")
                 _native_module = module
@@ -273,3 +278,193 @@ def quantize(x, out_dtype=torch.float8_e4m3fn, mode=QUANT_PER_MATRIX, rows_conti
     check(load_library().qgemm_quantize(_dt(x), _dt(q, True), mode, x.data_ptr(), ld, rows, cols, q.data_ptr(),
                                         cols, scales.data_ptr(), rs, cs, _stream()))
     return q, scales
+
+
+# ---- layer norm, activations in 8 bits, weight gradients.  Tensors of any number of dimensions are rows of their last one; the rows have to lie
+# evenly spaced, their elements side by side.
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_CODES = (torch.int8, torch.float8_e4m3fn)
+
+
+def _rows_of(t, name):
+    """(rows, cols, ld) of a tensor as rows of its last dimension."""
+    _need_gpu(t)
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{name} must have a last dimension of one or more elements, got shape {tuple(t.shape)}")
+    cols, rows, step, even = t.shape[-1], 1, 0, t.shape[-1] == 1 or t.stride(-1) == 1
+    for n, stride in reversed(list(zip(t.shape[:-1], t.stride()[:-1]))):
+        if n == 1:
+            continue
+        if rows == 1:
+            step = stride
+        even = even and (rows == 1 or stride == rows * step)
+        rows *= n
+    if rows == 0:
+        return 0, cols, cols
+    ld = step if rows > 1 else cols
+    if not even or ld < cols:
+        raise ValueError(f"{name} must be rows of contiguous elements, evenly spaced, got shape {tuple(t.shape)} strides {t.stride()}")
+    return rows, cols, ld
+
+
+def _need_type(t, types, name):
+    dtype = t if isinstance(t, torch.dtype) else t.dtype
+    if dtype not in types:
+        raise TypeError(f"{name} must be one of {', '.join(str(x) for x in types)}, got {dtype}")
+
+
+def _need_floats(t, n, name):
+    _need_gpu(t)
+    _need_type(t, (torch.float32,), name)
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must hold {n} contiguous values, got shape {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _parameters(weight, bias, cols):
+    """(type, pointer, pointer) of a layer norm's parameters, one of which or both may be None."""
+    if weight is None:
+        if bias is not None:
+            raise ValueError("a bias needs a weight")
+        return DT_F32, None, None
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        _need_gpu(t)
+        _need_type(t, _FLOATS, name)
+        if t.numel() != cols or not t.is_contiguous() or t.dtype != weight.dtype:
+            raise ValueError(f"{name} must hold {cols} contiguous values of {weight.dtype}, got {t.dtype} {tuple(t.shape)}")
+    return _dt(weight), weight.data_ptr(), None if bias is None else bias.data_ptr()
+
+
+def _scales_like(t, cols):
+    return torch.empty((*t.shape[:-1], -(-cols // 128)), dtype=torch.float32, device=t.device)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None, keep=None):
+    """y, mean, rstd = layer norm of the rows of x [..., cols], fp32 / bf16 / fp16: y = xhat * weight + bias with xhat = (x - mean) * rstd,
+    rstd = 1 / sqrt(var + eps); weight and bias [cols], fp32 / bf16 / fp16, or None.  y has x's type, or out_dtype; mean and rstd are fp32.
+    keep (torch.int8 or torch.float8_e4m3fn): y, mean, rstd, q, scales, where q and scales are xhat in 8 bits as checkpoint() gives it: what
+    layer_norm_backward and weight_gradient need of this layer's activations."""
+    native = _native()
+    if native:
+        st, *out = native.ops_layer_norm(x, weight, bias, eps, out_dtype, keep)
+        if st == 0:
+            return tuple(out) if keep is not None else tuple(out[:3])
+        if st > 0:
+            check(st)
+    rows, cols, ld = _rows_of(x, "x")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    _need_type(x, _FLOATS, "x")
+    _need_type(out_dtype, _FLOATS, "out_dtype")
+    params, w, b = _parameters(weight, bias, cols)
+    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2))
+    q = scales = None
+    if keep is not None:
+        _need_type(keep, _CODES, "keep")
+        q, scales = torch.empty(x.shape, dtype=keep, device=x.device), _scales_like(x, cols)
+    check(load_library().qgemm_layer_norm(
+        _dt(x), _dt(y), params, DT_I8 if q is None else _dt(q), x.data_ptr(), ld, w, b, eps, y.data_ptr(), cols, mean.data_ptr(), rstd.data_ptr(),
+        None if q is None else q.data_ptr(), cols, None if q is None else scales.data_ptr(), rows, cols, _stream()))
+    return (y, mean, rstd) if keep is None else (y, mean, rstd, q, scales)
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, scales=None, bias=True, out_dtype=None):
+    """dx, dweight, dbias of layer_norm: dy [..., cols]; x is the norm's input, with its mean and rstd, or the codes q that
+    layer_norm(..., keep=...) gave, with their scales (mean may be None then).  dx has dy's type, or out_dtype; dweight and dbias have weight's, and
+    are None where weight is (dbias also with bias=False)."""
+    native = _native()
+    if native:
+        st, *out = native.ops_layer_norm_backward(dy, x, mean, rstd, weight, scales, bias, out_dtype)
+        if st == 0:
+            return tuple(out)
+        if st > 0:
+            check(st)
+    rows, cols, lddy = _rows_of(dy, "dy")
+    xrows, xcols, ldx = _rows_of(x, "x")
+    if (rows, cols) != (xrows, xcols):
+        raise ValueError(f"dy and x must have the same rows, got {tuple(dy.shape)} and {tuple(x.shape)}")
+    out_dtype = dy.dtype if out_dtype is None else out_dtype
+    _need_type(dy, _FLOATS, "dy")
+    _need_type(out_dtype, _FLOATS, "out_dtype")
+    _need_type(x, _FLOATS + _CODES, "x")
+    params, w, _ = _parameters(weight, None, cols)
+    if x.dtype in _CODES:
+        if scales is None:
+            raise ValueError("codes need their scales")
+        s, m = _need_floats(scales, rows * -(-cols // 128), "scales"), None
+    else:
+        if mean is None or scales is not None:
+            raise ValueError("x that is not in 8 bits needs its mean, and has no scales")
+        s, m = None, _need_floats(mean, rows, "mean")
+    r = _need_floats(rstd, rows, "rstd")
+    dx = torch.empty(dy.shape, dtype=out_dtype, device=dy.device)
+    dw = None if weight is None else torch.empty_like(weight)
+    db = None if weight is None or not bias else torch.empty_like(weight)
+    check(load_library().qgemm_layer_norm_backward(
+        _dt(dy), _dt(x), _dt(dx), params, dy.data_ptr(), lddy, x.data_ptr(), ldx, s, m, r, w, dx.data_ptr(), cols,
+        None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), rows, cols, _stream()))
+    return dx, dw, db
+
+
+def checkpoint(x, dtype=torch.int8):
+    """q, scales = an activation x [..., cols], fp32 / bf16 / fp16, in 8 bits for the backward pass: codes (torch.int8 or torch.float8_e4m3fn) and
+    one power of two for the 128 columns of a block, scales [..., ceil(cols/128)].  q * scale is exact in bf16."""
+    native = _native()
+    if native:
+        st, q, scales = native.ops_checkpoint(x, dtype)
+        if st == 0:
+            return q, scales
+        if st > 0:
+            check(st)
+    rows, cols, ld = _rows_of(x, "x")
+    _need_type(x, _FLOATS, "x")
+    _need_type(dtype, _CODES, "dtype")
+    q, scales = torch.empty(x.shape, dtype=dtype, device=x.device), _scales_like(x, cols)
+    check(load_library().qgemm_checkpoint(_dt(x), _dt(q), x.data_ptr(), ld, rows, cols, q.data_ptr(), cols, scales.data_ptr(), _stream()))
+    return q, scales
+
+
+def restore(q, scales, dtype=torch.bfloat16):
+    """The values that codes of checkpoint(), layer_norm(..., keep=...) or quantize(x, ..., QUANT_BLOCK_1x128) stand for."""
+    native = _native()
+    if native:
+        st, x = native.ops_restore(q, scales, dtype)
+        if st == 0:
+            return x
+        if st > 0:
+            check(st)
+    rows, cols, ld = _rows_of(q, "q")
+    _need_type(q, _CODES, "q")
+    _need_type(dtype, _FLOATS, "dtype")
+    s = _need_floats(scales, rows * -(-cols // 128), "scales")
+    x = torch.empty(q.shape, dtype=dtype, device=q.device)
+    check(load_library().qgemm_restore(_dt(q), _dt(x), q.data_ptr(), ld, s, rows, cols, x.data_ptr(), cols, _stream()))
+    return x
+
+
+def weight_gradient(dy, q, scales, weight=None, bias=None, out_dtype=torch.float32):
+    """dw [n, cols], db [n] (fp32) = the gradients of a linear layer z = v W^T + c: dw = dy^T v, db = the sums of dy over its rows.  dy [..., n] bf16 or fp16;
+    v is the layer's input in 8 bits, q [..., cols] and its scales.  With weight (and bias) q holds a layer norm's xhat, and
+    v = xhat * weight + bias is meant."""
+    native = _native()
+    if native:
+        st, dw, db = native.ops_weight_gradient(dy, q, scales, weight, bias, out_dtype)
+        if st == 0:
+            return dw, db
+        if st > 0:
+            check(st)
+    rows, n, lddy = _rows_of(dy, "dy")
+    qrows, cols, ldq = _rows_of(q, "q")
+    if rows != qrows:
+        raise ValueError(f"dy and q must have the same rows, got {tuple(dy.shape)} and {tuple(q.shape)}")
+    _need_type(dy, _FLOATS[1:], "dy")
+    _need_type(q, _CODES, "q")
+    _need_type(out_dtype, _FLOATS, "out_dtype")
+    params, w, b = _parameters(weight, bias, cols)
+    s = _need_floats(scales, rows * -(-cols // 128), "scales")
+    dw, db = torch.empty((n, cols), dtype=out_dtype, device=dy.device), torch.empty(n, dtype=torch.float32, device=dy.device)
+    check(load_library().qgemm_weight_gradient(_dt(dy), _dt(q), _dt(dw), params, dy.data_ptr(), lddy, q.data_ptr(), ldq, s, w, b, dw.data_ptr(), cols,
+                                               db.data_ptr(), rows, n, cols, _stream()))
+    return dw, db
