@@ -34,13 +34,20 @@ __device__ __forceinline__ void centre(float (&v)[8], float mean, uint32_t c, ui
 }
 
 // codes and scale of an octet of xhat, which holds zeros behind the row's end; all 16 lanes of a block come here
+template <int ROW = ROW_ANY>
 __device__ __forceinline__ void keep_octet(const NormArgs &p, uint32_t row, uint32_t c, const float (&xhat)[8]) {
-    const uint32_t m = block_max_bits(xhat);
+    float own[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) own[e] = xhat[e];
+    if (any_repeated<ROW>(c, p.cols))
+#pragma unroll
+        for (int e = 0; e < 8; ++e) own[e] = e < (int)repeated<ROW>(c, p.cols) ? 0.0f : own[e];
+    const uint32_t m = block_max_bits(own);
     const bool i8 = p.q_dt == QGEMM_DT_I8;
     const PowerOfTwo s = i8 ? power_of_two<QGEMM_DT_I8>(m) : power_of_two<QGEMM_DT_F8E4M3>(m);
     if (c >= p.cols) return;
     const v2i q = i8 ? octet_codes<QGEMM_DT_I8>(xhat, s.inv) : octet_codes<QGEMM_DT_F8E4M3>(xhat, s.inv);
-    store_codes((uint8_t *)p.q + (size_t)row * p.ldq, c, p.cols, q);
+    store_codes<ROW>((uint8_t *)p.q + (size_t)row * p.ldq, c, p.cols, q);
     if (c % kScaleBlock == 0) p.scales[(size_t)row * p.kb + c / kScaleBlock] = s.s;
 }
 
@@ -114,6 +121,138 @@ __global__ void __launch_bounds__(256) norm_any_kernel(const NormArgs p) {
     }
 }
 
+// ---- rows in registers: GROUP threads hold a row, P octets each, and read it once.
+// Statistics of a wave's part are exact to two passes (sum, then squares about its own mean), both in registers; parts of a row meet
+// once: with n_w elements, mean m_w and squares M_w of part w, sum (x - mean)^2 = sum M_w + n_w (m_w - mean)^2, which cancels nothing.
+// SAME: the parameters have x's type, else they are fp32.  AHEAD: an octet of them is requested in front of the one that is being worked
+// on, the first with the row: half a trip to memory less for a row by itself, and registers that many rows want for more waves
+// (us, without / with: 1 x 7168 bf16 4.3 / 3.9, 6144 x 7168 43.3 / 49.8).  ROW: see RowKind.
+template <int DT, int GROUP, int P, bool SAME, bool AHEAD, int ROW>
+__global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) norm_rows_kernel(const NormArgs p) {
+    constexpr int THREADS = GROUP < 256 ? 256 : GROUP, ROWS = THREADS / GROUP, WAVES = GROUP / 64, LANES = GROUP < 64 ? GROUP : 64;
+    typedef Octet<SAME ? DT : QGEMM_DT_F32> Param;
+    const uint32_t t = threadIdx.x % GROUP, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), cols = p.cols;
+    const float n = (float)cols;
+    auto column = [&](int i) { return (i * GROUP + t) * kOctet; };
+    int turn = 0;
+    for (uint32_t first = blockIdx.x * ROWS; first < p.rows; first += gridDim.x * ROWS, turn ^= 1) {
+        const uint32_t row = ROWS == 1 ? first : first + threadIdx.x / GROUP;
+        const bool in_rows = ROWS == 1 || row < p.rows;
+        const char *x = (const char *)p.x + (size_t)(in_rows ? row : p.rows - 1) * p.ldx * Octet<DT>::ES;
+        Octet<DT> o[P];
+        Param w[P], b[P];
+        auto parameters = [&](int i) {
+            if (p.weight) w[i].template request<ROW>(p.weight, column(i), cols);
+            if (p.bias) b[i].template request<ROW>(p.bias, column(i), cols);
+        };
+#pragma unroll
+        for (int i = 0; i < P; ++i) o[i].template request<ROW>(x, column(i), cols);
+        if (AHEAD) parameters(0);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float v[8];
+            o[i].template settle<ROW>(column(i), cols);
+            o[i].hold();
+            o[i].floats(v);
+            if (any_repeated<ROW>(column(i), cols))
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = e < (int)repeated<ROW>(column(i), cols) ? 0.0f : v[e];
+            sum += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        sum = lanes_sum<LANES>(sum);
+        float part = n;                                      // elements of the row in this wave
+        if constexpr (WAVES > 1) {
+            uint32_t have = 0;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const uint32_t from = (i * GROUP + wave * 64) * kOctet;
+                have += from < cols ? (cols - from < 512 ? cols - from : 512) : 0;
+            }
+            part = (float)have;
+        }
+        float mean = WAVES > 1 && part == 0.0f ? 0.0f : sum / part, squares = 0.0f;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const uint32_t c = column(i);
+            float v[8];
+            o[i].hold();
+            o[i].floats(v);
+            float s = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] -= mean;
+            if (any_repeated<ROW>(c, cols))
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = e < (int)repeated<ROW>(c, cols) ? 0.0f : v[e];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += v[e] * v[e];
+            squares += c < cols ? s : 0.0f;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        squares = lanes_sum<LANES>(squares);
+        if constexpr (WAVES > 1) {
+            __shared__ float red[2][WAVES][3];
+            if ((threadIdx.x & 63) == 0) {
+                red[turn][wave][0] = sum;
+                red[turn][wave][1] = squares;
+                red[turn][wave][2] = part;
+            }
+            __syncthreads();
+            float all = 0.0f;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) all += red[turn][i][0];
+            mean = all / n;
+            squares = 0.0f;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) {
+                const float k = red[turn][i][2], d = k == 0.0f ? 0.0f : red[turn][i][0] / k - mean;
+                squares += red[turn][i][1] + k * (d * d);
+            }
+        }
+        const float rstd = 1.0f / __builtin_sqrtf(squares / n + p.eps);
+        if (t == 0 && in_rows) {
+            if (p.mean) p.mean[row] = mean;
+            if (p.rstd) p.rstd[row] = rstd;
+        }
+        char *y = (char *)p.y + (size_t)row * p.ldy * dtype_bytes(p.y_dt);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const uint32_t c = column(i);
+            float v[8];
+            if (AHEAD && i + 1 < P) parameters(i + 1);
+            o[i].hold();
+            o[i].floats(v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (v[e] - mean) * rstd;
+            if (p.q) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = c < cols ? v[e] : 0.0f;
+                if (in_rows) keep_octet<ROW>(p, row, c, v);
+            }
+            if (in_rows && c < cols) {
+                float f[8];
+                if (p.weight) {
+                    if (!AHEAD) w[i].template request<ROW>(p.weight, c, cols);
+                    w[i].template settle<ROW>(c, cols);
+                    w[i].floats(f);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] *= f[e];
+                }
+                if (p.bias) {
+                    if (!AHEAD) b[i].template request<ROW>(p.bias, c, cols);
+                    b[i].template settle<ROW>(c, cols);
+                    b[i].floats(f);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += f[e];
+                }
+                store_octet<ROW>(y, p.y_dt, c, cols, v);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+}
+
 // ---- backward
 // xhat of an octet: out of x, or codes times their scale
 template <int X_DT>
@@ -121,12 +260,16 @@ struct Normalised {
     static constexpr bool CODES = X_DT == QGEMM_DT_I8 || X_DT == QGEMM_DT_F8E4M3;
     Octet<X_DT> o;
     float scale;
+    template <int ROW = ROW_ANY>
     __device__ __forceinline__ void request(const NormBackwardArgs &p, uint32_t row, uint32_t c) {
-        o.request((const char *)p.x + (size_t)row * p.ldx * Octet<X_DT>::ES, c, p.cols);
+        o.template request<ROW>((const char *)p.x + (size_t)row * p.ldx * Octet<X_DT>::ES, c, p.cols);
         if constexpr (CODES) scale = p.scales[(size_t)row * p.kb + (c < p.cols ? c / kScaleBlock : 0)];
     }
-    __device__ __forceinline__ void values(const NormBackwardArgs &p, uint32_t c, float mean, float rstd, float (&v)[8]) {
-        o.settle(c, p.cols);
+    template <int ROW = ROW_ANY>
+    __device__ __forceinline__ void settle(uint32_t c, uint32_t cols) {
+        o.template settle<ROW>(c, cols);
+    }
+    __device__ __forceinline__ void values(float mean, float rstd, float (&v)[8]) const {
         o.floats(v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = CODES ? v[e] * scale : (v[e] - mean) * rstd;
@@ -148,7 +291,8 @@ __global__ void __launch_bounds__(256) norm_backward_any_kernel(const NormBackwa
             n.request(p, row, c);
             o.settle(c, p.cols);
             o.floats(g);
-            n.values(p, c, mean, rstd, xhat);
+            n.settle(c, p.cols);
+            n.values(mean, rstd, xhat);
             if (p.weight) {
                 float w[8];
                 parameter_octet(p.weight, p.param_dt, c, p.cols, w);
@@ -177,6 +321,156 @@ __global__ void __launch_bounds__(256) norm_backward_any_kernel(const NormBackwa
     }
 }
 
+// Rows in registers: GROUP threads hold a row of dy and of x, P octets each; a workgroup goes over its rows with the next one's
+// loads in flight, and keeps the sums of its columns in registers until the end.
+template <int DY_DT, int X_DT, int GROUP, int P, int ROW>
+__global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) norm_backward_rows_kernel(const NormBackwardArgs p) {
+    constexpr int THREADS = GROUP < 256 ? 256 : GROUP, ROWS = THREADS / GROUP, WAVES = GROUP / 64, LANES = GROUP < 64 ? GROUP : 64;
+    constexpr bool CODES = Normalised<X_DT>::CODES;
+    const uint32_t t = threadIdx.x % GROUP, sub = ROWS == 1 ? 0 : threadIdx.x / GROUP, cols = p.cols;
+    const float n = (float)cols;
+    const bool sums = p.dweight || p.dbias;
+    auto column = [&](int i) { return (i * GROUP + t) * kOctet; };
+    struct Row {
+        Octet<DY_DT> dy[P];
+        Normalised<X_DT> x[P];
+        float mean, rstd;
+    };
+    auto fetch = [&](Row &r, uint32_t first) {
+        uint32_t row = first + sub;
+        if (ROWS > 1) row = row < p.rows ? row : p.rows - 1;
+        const char *dy = (const char *)p.dy + (size_t)row * p.lddy * Octet<DY_DT>::ES;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            r.dy[i].template request<ROW>(dy, column(i), cols);
+            r.x[i].template request<ROW>(p, row, column(i));
+        }
+        r.rstd = p.rstd[row];
+        r.mean = CODES ? 0.0f : p.mean[row];
+    };
+    float w[P][8], dw[P][8] = {}, db[P][8] = {};
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        if (p.weight) parameter_octet<ROW>(p.weight, p.param_dt, column(i), cols, w[i]);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[i][e] = 1.0f;
+    }
+    Row next;
+    const uint32_t stride = gridDim.x * ROWS;
+    fetch(next, blockIdx.x * ROWS);
+    int turn = 0;
+    for (uint32_t first = blockIdx.x * ROWS; first < p.rows; first += stride, turn ^= 1) {
+        Row r = next;
+        const bool in_rows = ROWS == 1 || first + sub < p.rows;
+        if (p.rows - first > stride) fetch(next, first + stride);
+        float a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float g[8], xhat[8];
+            r.dy[i].template settle<ROW>(in_rows ? column(i) : cols, cols);
+            r.x[i].template settle<ROW>(column(i), cols);
+            r.dy[i].hold();
+            r.x[i].o.hold();
+            r.dy[i].floats(g);
+            r.x[i].values(r.mean, r.rstd, xhat);
+            if (any_repeated<ROW>(column(i), cols))
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[e] = e < (int)repeated<ROW>(column(i), cols) ? 0.0f : g[e];
+            if (sums) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    dw[i][e] += g[e] * xhat[e];
+                    db[i][e] += g[e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                g[e] *= w[i][e];
+                a += g[e];
+                b += g[e] * xhat[e];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        a = lanes_sum<LANES>(a);
+        b = lanes_sum<LANES>(b);
+        if constexpr (WAVES > 1) {
+            __shared__ float red[2][2][WAVES];
+            if ((threadIdx.x & 63) == 0) {
+                red[turn][0][threadIdx.x >> 6] = a;
+                red[turn][1][threadIdx.x >> 6] = b;
+            }
+            __syncthreads();
+            a = red[turn][0][0];
+            b = red[turn][1][0];
+#pragma unroll
+            for (int i = 1; i < WAVES; ++i) {
+                a += red[turn][0][i];
+                b += red[turn][1][i];
+            }
+        }
+        a /= n;
+        b /= n;
+        char *dx = (char *)p.dx + (size_t)(first + sub) * p.lddx * dtype_bytes(p.dx_dt);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float g[8], xhat[8];
+            r.dy[i].hold();
+            r.x[i].o.hold();
+            r.dy[i].floats(g);
+            r.x[i].values(r.mean, r.rstd, xhat);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[e] = r.rstd * (g[e] * w[i][e] - a - xhat[e] * b);
+            if (in_rows && column(i) < cols) store_octet<ROW>(dx, p.dx_dt, column(i), cols, g);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    if (!sums) return;
+    float *out = p.partial + (size_t)blockIdx.x * 2 * norm_partial_cols(cols);
+    if constexpr (ROWS == 1) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if (column(i) >= cols) continue;
+            if (const uint32_t before = repeated<ROW>(column(i), cols)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (e < (int)before) continue;
+                    out[column(i) - before + e] = dw[i][e];
+                    out[norm_partial_cols(cols) + column(i) - before + e] = db[i][e];
+                }
+                continue;
+            }
+            v4f *at = (v4f *)(out + column(i)), *bt = (v4f *)(out + norm_partial_cols(cols) + column(i));
+            at[0] = v4f{dw[i][0], dw[i][1], dw[i][2], dw[i][3]};
+            at[1] = v4f{dw[i][4], dw[i][5], dw[i][6], dw[i][7]};
+            bt[0] = v4f{db[i][0], db[i][1], db[i][2], db[i][3]};
+            bt[1] = v4f{db[i][4], db[i][5], db[i][6], db[i][7]};
+        }
+    } else {
+        __shared__ float fold[THREADS * 8];                     // [ROWS][GROUP * 8]
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int before = (int)repeated<ROW>(column(i), cols);
+                    if (ROW != ROW_RAGGED || e >= before) fold[threadIdx.x * 8 + e - before] = which ? db[i][e] : dw[i][e];
+                }
+                __syncthreads();
+#pragma unroll 1
+                for (uint32_t c = threadIdx.x; c < GROUP * 8; c += THREADS) {
+                    float s = fold[c];
+#pragma unroll
+                    for (int k = 1; k < ROWS; ++k) s += fold[k * GROUP * 8 + c];
+                    if (i * GROUP * 8 + c < cols) out[which * norm_partial_cols(cols) + i * GROUP * 8 + c] = s;
+                }
+            }
+        }
+    }
+}
+
 // column sums over the rows of a slice: 128 columns a workgroup, 16 rows at a time
 template <int DY_DT, int X_DT>
 __global__ void __launch_bounds__(256) norm_column_sums_kernel(const NormBackwardArgs p) {
@@ -192,14 +486,15 @@ __global__ void __launch_bounds__(256) norm_column_sums_kernel(const NormBackwar
         n.request(p, row, c);
         o.settle(c, p.cols);
         o.floats(dy);
-        n.values(p, c, mean, rstd, xhat);
+        n.settle(c, p.cols);
+        n.values(mean, rstd, xhat);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             dw[e] += dy[e] * xhat[e];
             db[e] += dy[e];
         }
     }
-    const size_t stride = ((size_t)p.cols + 63) / 64 * 64;
+    const size_t stride = norm_partial_cols(p.cols);
     float *out = p.partial + (size_t)blockIdx.y * 2 * stride;
     for (int which = 0; which < 2; ++which) {
         __syncthreads();
@@ -215,23 +510,41 @@ __global__ void __launch_bounds__(256) norm_column_sums_kernel(const NormBackwar
     }
 }
 
-// dweight / dbias out of the workgroups' sums: 64 columns a workgroup, always in the same order.  blockIdx.y: which of the two
-__global__ void __launch_bounds__(256) norm_parameter_sums_kernel(const NormBackwardArgs p) {
-    __shared__ float red[16][64];
-    const size_t stride = ((size_t)p.cols + 63) / 64 * 64;
-    const uint32_t lane = threadIdx.x & 15, sub = threadIdx.x >> 4, which = blockIdx.y;
+// dweight / dbias out of the workgroups' sums: 32 columns a workgroup, 64 partial sums at a time, eight of which a lane has in flight, always in
+// the same order.  blockIdx.y: which of the two
+__global__ void __launch_bounds__(512) norm_parameter_sums_kernel(const NormBackwardArgs p) {
+    constexpr uint32_t SLICES = 64, DEEP = 8;
+    __shared__ v4f red[SLICES][8];
+    const size_t stride = norm_partial_cols(p.cols);
+    const uint32_t lane = threadIdx.x & 7, sub = threadIdx.x >> 3, which = blockIdx.y;
     void *out = which ? p.dbias : p.dweight;
     if (!out) return;
-    const float *in = p.partial + which * stride + (size_t)blockIdx.x * 64 + lane * 4;
+    const float *in = p.partial + which * stride + (size_t)blockIdx.x * 32 + lane * 4;
     v4f s = v4f{0, 0, 0, 0};
-    for (uint32_t g = sub; g < p.groups; g += 16) s += *(const v4f *)(in + (size_t)g * 2 * stride);
-    *(v4f *)&red[sub][lane * 4] = s;
-    __syncthreads();
-    const uint32_t c = blockIdx.x * 64 + threadIdx.x;
-    if (threadIdx.x >= 64 || c >= p.cols) return;
-    float v = red[0][threadIdx.x];
+    for (uint32_t g = sub; g < p.groups; g += SLICES * DEEP) {
+        v4f v[DEEP];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += red[i][threadIdx.x];
+        for (uint32_t i = 0; i < DEEP; ++i) {
+            const uint32_t at = g + i * SLICES;
+            v[i] = *(const v4f *)(in + (size_t)(at < p.groups ? at : g) * 2 * stride);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < DEEP; ++i)
+            if (g + i * SLICES < p.groups) s += v[i];
+    }
+    red[sub][lane] = s;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t half = SLICES / 2; half >= 8; half /= 2) {
+        if (sub < half) red[sub][lane] += red[sub + half][lane];
+        __syncthreads();
+    }
+    const uint32_t c = blockIdx.x * 32 + threadIdx.x;
+    if (threadIdx.x >= 32 || c >= p.cols) return;
+    const float *at = (const float *)red + threadIdx.x;
+    float v = at[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v += at[i * 32];
     if (p.param_dt == QGEMM_DT_F32) ((float *)out)[c] = v;
     else ((uint16_t *)out)[c] = p.param_dt == QGEMM_DT_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
 }

@@ -7,18 +7,41 @@ namespace qgemm {
 
 constexpr uint32_t kOctet = 8;
 
-// the last octet of a row that ends inside it is fetched whole from where it still lies in the row, and moved down afterwards: no lane
-// reads behind a row, and nothing branches between the loads.  Rows of fewer than eight elements are fetched one by one.
+// What is known of a row's length: anything; eight elements or more, of fewer than 2^32 bytes; the same, a multiple of eight
+enum RowKind : int { ROW_ANY = 0, ROW_RAGGED = 1, ROW_WHOLE = 2 };
+template <int ROW>
+using row_offset = std::conditional_t<ROW == ROW_ANY, size_t, uint32_t>;
+
+// A row that ends inside its last octet: no lane reads behind it, and nothing branches between loads, as the last eight elements are
+// fetched from where they lie.
+//   ROW_RAGGED  the lane works on those eight: the first `repeated` of them are the octet in front's as well, count in no sum and are
+//               written twice, with the same values.  (Moving them down instead, and writing the end element by element, kept one wave of
+//               every row a third longer than the others: norm of 4096 x 3001 bf16 19.1 us, 14.2 for 3000)
+//   ROW_ANY     they are moved down, zeros behind them; rows of fewer than eight are fetched one by one
+template <int ROW>
+__device__ __forceinline__ uint32_t octet_begin(uint32_t c, uint32_t cols) {
+    return ROW == ROW_RAGGED && c < cols && cols - c < kOctet ? cols - kOctet : c;
+}
+// how many elements in front of column c the octet of a lane starts, and whether any lane of the wave has such
+template <int ROW>
+__device__ __forceinline__ uint32_t repeated(uint32_t c, uint32_t cols) {
+    return c - octet_begin<ROW>(c, cols);
+}
+template <int ROW>
+__device__ __forceinline__ bool any_repeated(uint32_t c, uint32_t cols) {
+    return ROW == ROW_RAGGED && __any(repeated<ROW>(c, cols) != 0);
+}
 template <int DT>
 struct Octet {
     static constexpr int ES = DT == QGEMM_DT_F32 ? 4 : (DT == QGEMM_DT_BF16 || DT == QGEMM_DT_F16) ? 2 : 1, DW = 2 * ES;
     uint32_t w[DW];
 
     // elements c .. c + 7 of a row of `cols`, as they come from memory; `settle` brings them in order
+    template <int ROW = ROW_ANY>
     __device__ __forceinline__ void request(const void *row, uint32_t c, uint32_t cols) {
         const char *p = (const char *)row;
-        if (cols >= kOctet) {
-            p += (size_t)(c < cols - kOctet ? c : cols - kOctet) * ES;
+        if (ROW != ROW_ANY || cols >= kOctet) {
+            p += (row_offset<ROW>)(c < cols - kOctet ? c : cols - kOctet) * ES;
             if constexpr (DW == 2) {
                 const v2i v = *(const v2i_any *)p;
                 w[0] = v[0], w[1] = v[1];
@@ -34,15 +57,21 @@ struct Octet {
             few(p, c < cols ? cols - c : 0);
         }
     }
-    // zeros behind the row's end
+    // zeros where the row has nothing
+    template <int ROW = ROW_ANY>
     __device__ __forceinline__ void settle(uint32_t c, uint32_t cols) {
         const bool in = c < cols;
-        if (cols >= kOctet && cols % kOctet != 0) {
+        if (ROW == ROW_ANY && cols >= kOctet) {
             const uint32_t gone = in && c > cols - kOctet ? c - (cols - kOctet) : 0;
             if (__any(gone != 0)) move_down<DW, ES == 4>(w, gone * ES);
         }
 #pragma unroll
         for (int i = 0; i < DW; ++i) w[i] = in ? w[i] : 0;
+    }
+    // (the compiler converts again what it would otherwise keep as floats, in up to four times the registers)
+    __device__ __forceinline__ void hold() {
+#pragma unroll
+        for (int i = 0; i < DW; ++i) asm volatile("" : "+v"(w[i]));
     }
     __device__ __forceinline__ void floats(float (&v)[8]) const {
         if constexpr (DT == QGEMM_DT_F32) {
@@ -90,10 +119,11 @@ private:
 };
 
 // the same of a type that is known to the launch only (parameters: fp32, bf16 or fp16)
+template <int ROW = ROW_ANY>
 __device__ __forceinline__ void parameter_octet(const void *p, int dt, uint32_t c, uint32_t cols, float (&v)[8]) {
     auto take = [&](auto o) {
-        o.request(p, c, cols);
-        o.settle(c, cols);
+        o.template request<ROW>(p, c, cols);
+        o.template settle<ROW>(c, cols);
         o.floats(v);
     };
     if (dt == QGEMM_DT_F32) take(Octet<QGEMM_DT_F32>());
@@ -102,16 +132,18 @@ __device__ __forceinline__ void parameter_octet(const void *p, int dt, uint32_t 
 }
 
 // v as elements c .. c + 7 of a row of `cols` (c < cols), one rounding to nearest even where the type has fewer bits
+template <int ROW = ROW_ANY>
 __device__ __forceinline__ void store_octet(void *row, int dt, uint32_t c, uint32_t cols, const float (&v)[8]) {
-    if (cols - c >= kOctet) {
+    if (ROW == ROW_RAGGED) c = octet_begin<ROW>(c, cols);
+    if (ROW != ROW_ANY || cols - c >= kOctet) {
         if (dt == QGEMM_DT_F32) {
-            v4f_any *p = (v4f_any *)((float *)row + c);
+            v4f_any *p = (v4f_any *)((char *)row + (row_offset<ROW>)c * 4);
             p[0] = v4f{v[0], v[1], v[2], v[3]};
             p[1] = v4f{v[4], v[5], v[6], v[7]};
         } else {
             const v2i a = dt == QGEMM_DT_BF16 ? pack4_bf16(v[0], v[1], v[2], v[3]) : pack4_f16(v[0], v[1], v[2], v[3]);
             const v2i b = dt == QGEMM_DT_BF16 ? pack4_bf16(v[4], v[5], v[6], v[7]) : pack4_f16(v[4], v[5], v[6], v[7]);
-            *(v4i_any *)((uint16_t *)row + c) = v4i{a[0], a[1], b[0], b[1]};
+            *(v4i_any *)((char *)row + (row_offset<ROW>)c * 2) = v4i{a[0], a[1], b[0], b[1]};
         }
         return;
     }
@@ -122,15 +154,22 @@ __device__ __forceinline__ void store_octet(void *row, int dt, uint32_t c, uint3
         else ((uint16_t *)row)[c + e] = dt == QGEMM_DT_BF16 ? f32_to_bf16_bits(v[e]) : f32_to_f16_bits(v[e]);
     }
 }
+template <int ROW = ROW_ANY>
 __device__ __forceinline__ void store_codes(void *row, uint32_t c, uint32_t cols, v2i q) {
     uint8_t *p = (uint8_t *)row + c;
-    if (cols - c >= kOctet) {
+    if (ROW == ROW_WHOLE || cols - c >= kOctet) {
         *(v2i_any *)p = q;
         return;
     }
+    const uint32_t before = repeated<ROW>(c, cols);
+    if (ROW == ROW_RAGGED && c % kScaleBlock != 0) {          // (what is repeated lies under the same scale)
+        *(v2i_any *)(p - before) = q;
+        return;
+    }
+    const uint64_t all = ((uint64_t)(uint32_t)q[1] << 32 | (uint32_t)q[0]) >> (8 * before);
 #pragma unroll
     for (int e = 0; e < 7; ++e)
-        if (e < (int)(cols - c)) p[e] = (uint8_t)((uint32_t)q[e >> 2] >> (8 * (e & 3)));
+        if (e < (int)(cols - c)) p[e] = (uint8_t)(all >> (8 * e));
 }
 
 // Sum over groups of 16, 32 or 64 neighbouring lanes, in every lane and in the same order whatever the lane (see lanes_max)

@@ -26,7 +26,7 @@ struct NormBackwardArgs {
 };
 // workgroups whose column sums a launch leaves in `partial`, 0 where nobody wants sums or there are no rows
 uint32_t norm_backward_groups(const NormBackwardArgs &a, int cus);
-inline size_t norm_partial_cols(uint32_t cols) { return ((size_t)cols + 63) / 64 * 64; }
+__host__ __device__ inline size_t norm_partial_cols(uint32_t cols) { return ((size_t)cols + 63) / 64 * 64; }
 inline size_t norm_partial_bytes(uint32_t groups, uint32_t cols) { return (size_t)groups * 2 * norm_partial_cols(cols) * sizeof(float); }
 hipError_t launch_layer_norm_backward(const NormBackwardArgs &a, int cus, hipStream_t stream);
 

@@ -279,8 +279,12 @@ def test_offsets_beyond_32_bits():
     x[-5:] = tail
     w, b = params_of(cols, F32, 43)
     y, mean, rstd, q, s = Q.layer_norm(x, w, b, keep=I8)
-    want = Q.layer_norm(tail, w, b, keep=I8)
-    assert all(np.array_equal(R.f64(a[-5:]), R.f64(c)) for a, c in zip((y, mean, rstd, q, s), want))
+    (ry, rm, rr, rx), (ey, em, er, ex) = R.norm(R.f64(tail), R.f64(w), R.f64(b), EPS)
+    R.check(y[-5:], ry, R.stored(ey, ry, BF16), "y")
+    R.check(mean[-5:], rm, em + R.U * np.abs(rm), "mean")
+    R.check(rstd[-5:], rr, er, "rstd")
+    R.check(torch.from_numpy(R.values(q[-5:], s[-5:])), rx, np.repeat(R.f64(s[-5:]), 128, 1)[:, :cols] / 2 + 2 * ex, "kept")
+    want = (None, None, rstd[-5:].clone(), q[-5:].clone(), s[-5:].clone())
     del y
     dy = x
     dx, dw, db = Q.layer_norm_backward(dy, q, None, rstd, w, scales=s)
