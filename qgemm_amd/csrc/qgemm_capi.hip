@@ -1807,7 +1807,7 @@ uint32_t blocks_of(size_t cols) { return (uint32_t)((cols + kScaleBlock - 1) / k
 // Body of qgemm_checkpoint (`encode`) and qgemm_restore
 int keep_entry(bool encode, int in_dt, int out_dt, const void *in, size_t ld_in, void *out, size_t ld_out, float *scales, size_t rows, size_t cols,
                void *stream) {
-    if (rows >= ((size_t)1 << 31) || cols >= ((size_t)1 << 31)) return QGEMM_ERR_TOO_LARGE;
+    if (rows >= ((size_t)1 << 31) || cols >= (size_t)kMaxGridY * 2048) return QGEMM_ERR_TOO_LARGE;      // (columns are the y extent of a launch)
     if (rows == 0 || cols == 0) return QGEMM_OK;
     if (!in || !out || !scales || ld_in < cols || ld_out < cols) return QGEMM_ERR_INVALID_ARG;
     std::lock_guard<std::mutex> lock(g_ctx.mu);
@@ -2170,6 +2170,7 @@ QGEMM_EXPORT int qgemm_weight_gradient(int dy_dtype, int q_dtype, int dw_dtype, 
     if (weight && !is_float_type(param_dtype)) return QGEMM_ERR_UNSUPPORTED;
     if (cols == 0 || (bias && !weight)) return QGEMM_ERR_INVALID_ARG;
     if (rows >= ((size_t)1 << 31) || n >= ((size_t)1 << 31) || cols >= ((size_t)1 << 31)) return QGEMM_ERR_TOO_LARGE;
+    if (((n + 127) / 128) * ((cols + 127) / 128) >= ((size_t)1 << 23)) return QGEMM_ERR_TOO_LARGE;       // (2^32 threads of the smallest tile)
     if (n == 0) return QGEMM_OK;
     if (!dw || lddw < cols || (rows && (!dy || !q || !scales || lddy < n || ldq < cols))) return QGEMM_ERR_INVALID_ARG;
     hipStream_t stream = (hipStream_t)stream_;
@@ -2185,12 +2186,13 @@ QGEMM_EXPORT int qgemm_weight_gradient(int dy_dtype, int q_dtype, int dw_dtype, 
     a.lddy = lddy, a.ldq = ldq, a.lddw = lddw;
     a.rows = (uint32_t)rows, a.n = (uint32_t)n, a.cols = (uint32_t)cols, a.kb = blocks_of(cols);
     a.dy_dt = dy_dtype, a.q_dt = q_dtype, a.param_dt = param_dtype, a.dw_dt = dw_dtype;
-    if (const size_t room = weight_grad_room(a, g_ctx.num_cus)) {
+    if (const size_t room = plan_weight_grad(a, g_ctx.num_cus)) {
         st = ensure_workspace_locked(room, stream, &a.room);
         if (st != QGEMM_OK) return st;
     }
-    g_ctx.last_config = "weight_gradient";
-    return launch_weight_grad(a, g_ctx.num_cus, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+    g_ctx.last_config = a.tile == TILE_256x256 ? "weight_gradient_256x256" : a.tile == TILE_256x128 ? "weight_gradient_256x128" : "weight_gradient_128x128";
+    if (a.slices > 1) g_ctx.last_config += "_split" + std::to_string(a.slices);
+    return launch_weight_grad(a, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
 }
 
 QGEMM_EXPORT int qgemm_gemm(int in_dtype, int out_dtype, int layout_b, const void *A, size_t ldA, const void *B, size_t ldB,

@@ -46,12 +46,19 @@ struct WeightGradArgs {
     const float *scales;
     void *dw;                               // n x cols
     float *db;                              // n, or null
-    void *room;                             // partial sums, weight_grad_room(...)
+    void *room;                             // the slices' partial sums
     uint64_t lddy, ldq, lddw;
     uint32_t rows, n, cols, kb;
     int dy_dt, q_dt, param_dt, dw_dt;
+    int tile;                               // GradTile
+    uint32_t slices, slice;                 // slices of the rows, and rows of one, a multiple of kGradStep
+    int plain;                              // octets of a step may be fetched by 32-bit offsets, as they lie
 };
-size_t weight_grad_room(const WeightGradArgs &a, int cus);
-hipError_t launch_weight_grad(const WeightGradArgs &a, int cus, hipStream_t stream);
+enum GradTile : int { TILE_128x128, TILE_256x128, TILE_256x256, GRAD_TILES };
+// partial sums of a slice: n of dy, then n rows of dW
+__host__ __device__ inline size_t grad_round(uint32_t v) { return ((size_t)v + 3) / 4 * 4; }
+__host__ __device__ inline size_t grad_plane(uint32_t n, uint32_t cols) { return grad_round(n) + n * grad_round(cols); }
+size_t plan_weight_grad(WeightGradArgs &a, int cus);          // chooses tile and slices; bytes of `room`
+hipError_t launch_weight_grad(const WeightGradArgs &a, hipStream_t stream);
 
 }  // namespace qgemm

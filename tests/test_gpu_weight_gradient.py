@@ -93,6 +93,30 @@ def test_special_values_stay_where_they_belong(rows, n, cols):
     assert torch.isnan(dw[:, :edge]).all() and torch.isfinite(dw[:, edge:]).all()
 
 
+@pytest.mark.parametrize("rows,n,cols,config", [(999, 8190, 1021, "256x128"), (2048, 2047, 7168, "256x256"), (4000, 512, 1030, "128x128_split"),
+                                                (16384, 1024, 4095, "256x256_split"), (32700, 512, 1020, "256x128_split"), (700, 1024, 1024, "128x128")])
+@pytest.mark.parametrize("dtype,codes,norm,out", [(BF16, I8, True, F32), (F16, F8, False, BF16)])
+def test_every_tile(rows, n, cols, config, dtype, codes, norm, out):
+    """Sizes that the tiles are chosen for, whole and split, against the formula in 64 bits on the GPU."""
+    say("weight_gradient tiles", rows, n, cols, dtype, codes, norm, out)
+    dy, q, s, w, b = operands(rows, n, cols, dtype, codes, norm, rows + n)
+    dw, db = Q.weight_gradient(dy, q, s, w, b, out_dtype=out)
+    assert Q.last_config().startswith("weight_gradient_" + config)
+    v = q.double() * s.double().repeat_interleave(128, 1)[:, :cols]
+    d = dy.double()
+    adds = (rows / 4 + 48) * R.U                          # as in training_ref.weight_gradient
+    ref, bound = torch.mm(d.t().contiguous(), v), adds * torch.mm(d.t().contiguous().abs(), v.abs())
+    sums, e_sums = d.sum(0), adds * d.abs().sum(0)
+    assert ((db.double() - sums).abs() <= e_sums + R.U * sums.abs()).all()
+    if norm:
+        w, b = w.double(), b.double()
+        scaled, rank1 = ref * w, sums[:, None] * b
+        bound = bound * w.abs() + 2 * R.U * scaled.abs() + e_sums[:, None] * b.abs() + 2 * R.U * ((scaled + rank1).abs() + 2 * rank1.abs())
+        ref = scaled + rank1
+    bound = bound * (1 + R.HALF_STEP[out]) + R.HALF_STEP[out] * ref.abs() + R.LEAST[out]
+    assert ((dw.double() - ref).abs() <= bound).all()
+
+
 def test_scales_that_are_no_powers_of_two():
     """q s is rounded to dy's type then: half a last place of each value more."""
     say("weight_gradient quantize scales")
