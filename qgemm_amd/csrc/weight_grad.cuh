@@ -6,12 +6,12 @@
 // into LDS as it is, codes are widened to dy's type on the way (exact where scales are powers of two: the only rounding there is otherwise), and
 // the matrix cores' operands, which run along the rows, are taken out of both with transposing reads.  fp32 accumulators, fp32 planes.
 //
-// What bounds it: at 8192 x 8192 x 4096 (bf16, int8 codes) 495 - 520 us, 1.06 - 1.11 PFLOP/s of the 1.54 that the product of two bf16 matrices
+// What bounds it: at 8192 x 8192 x 4096 (bf16, int8 codes) 480 - 510 us, 1.08 - 1.14 PFLOP/s of the 1.54 that the product of two bf16 matrices
 // reaches at 8192^3 on the same card.  Steps to there, us: waves that load, convert and multiply in turn, 128 x 128 tiles 1118, 256 x 256 610;
 // conversions between the products and buffers of four steps 570; waves of their own for copies and conversions 522; those in two pairs that work on
-// alternate steps 507.  Without any copying the computing waves take 405, without LDS reads as well 313; one computing wave a SIMD with 128 x 128 of
-// its own took 832 (nothing hides what it waits for).  Converting costs the copying waves 2.5 vector instructions an element, which
-// go between products that hold the same port: without them 470.
+// alternate steps 507; both operands in both of a pair's turns 485.  Without any copying the computing waves take 405, without LDS reads as well
+// 313; one computing wave a SIMD with 128 x 128 of its own took 832 (nothing hides what it waits for).  Converting costs the copying waves 2.5
+// vector instructions an element, which go between products that hold the same port: without them 470.
 #pragma once
 #include "octet.cuh"
 #include "training.h"
@@ -35,8 +35,9 @@ struct GradCfg {
     static constexpr int STAGE = (BN + BK) / 64 * PANEL;
     static constexpr int STAGES = 4, RING = STAGES * STAGE, LDS = RING + BN * 4;   // and a float for each row of the tile
     static constexpr int PASSES = (BN * BK * 4 + RING - 1) / RING, PASS_ROWS = BN / PASSES;      // the tile leaves through the ring
-    static constexpr int AHEAD = 2, Y = AHEAD + 1;                                 // fragments of dy are read AHEAD in front of their products
-    static_assert(BN % 64 == 0 && BK % 64 == 0 && LOAD_N >= 1 && LOAD_K >= 1, "whole panels");
+    static constexpr int AHEAD = 2;                                                // fragments of dy that are read in front of their products
+    static constexpr bool EVEN = BN * BK > 256 * 128;                              // both of a step's turns bring some of both operands
+    static_assert(BN % 64 == 0 && BK % 64 == 0 && LOAD_N % 2 == 0 && LOAD_K % 2 == 0, "whole panels, two halves");
     static_assert(BN % PASSES == 0 && PASS_ROWS % (BN / WN) == 0 && THREADS % (BK / 4) == 0, "whole waves in a pass, whole rows in a turn");
     static_assert(COPY % (BN / 8) == 0 && COPY % (BK / 8) == 0, "a lane's octets lie under one another");
 };
@@ -106,37 +107,37 @@ __global__ void __launch_bounds__(C::THREADS) weight_grad_kernel(const WeightGra
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>((const char *)at + bytes), 0, 0x7FFFFFFF, 0x00020000);
     };
     const uint32_t next_n = (uint32_t)(ROWS_N * p.lddy * 2), next_k = (uint32_t)(ROWS_K * p.ldq), next_s = ROWS_K * p.kb * 4;
-    auto plain_n = [&](Set &r, uint32_t m0) ALWAYS_INLINE {
+    auto plain_n = [&](Set &r, int i0, int i1, uint32_t m0) ALWAYS_INLINE {
         const auto from = base(p.dy, (uint64_t)m0 * p.lddy * 2);
 #pragma unroll
-        for (int i = 0; i < C::LOAD_N; ++i) {
+        for (int i = i0; i < i1; ++i) {
             const v4i v = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(from, at_n, i * next_n, 0));
 #pragma unroll
             for (int e = 0; e < 4; ++e) r.on[i].w[e] = (uint32_t)v[e];
         }
     };
-    auto plain_k = [&](Set &r, uint32_t m0) ALWAYS_INLINE {
+    auto plain_k = [&](Set &r, int i0, int i1, uint32_t m0) ALWAYS_INLINE {
         const auto q = base(p.q, (uint64_t)m0 * p.ldq), s = base(p.scales, (uint64_t)m0 * p.kb * 4);
 #pragma unroll
-        for (int i = 0; i < C::LOAD_K; ++i) {
+        for (int i = i0; i < i1; ++i) {
             const v2i v = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(q, at_k, i * next_k, 0));
             r.ok[i].w[0] = (uint32_t)v[0], r.ok[i].w[1] = (uint32_t)v[1];
             r.scale[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(s, at_s, i * next_s, 0));
         }
     };
-    auto request_n = [&](Set &r, uint32_t m0) ALWAYS_INLINE {
-        if (m0 + kGradStep <= plain_to) return plain_n(r, m0);
+    auto request_n = [&](Set &r, int i0, int i1, uint32_t m0) ALWAYS_INLINE {
+        if (m0 + kGradStep <= plain_to) return plain_n(r, i0, i1, m0);
 #pragma unroll
-        for (int i = 0; i < C::LOAD_N; ++i) {
+        for (int i = i0; i < i1; ++i) {
             const uint32_t m = m0 + row_n + i * ROWS_N;
             r.on[i].request((const char *)p.dy + (size_t)(m < to ? m : p.rows - 1) * p.lddy * 2, cn, p.n);
             r.on[i].settle(m < to ? cn : p.n, p.n);
         }
     };
-    auto request_k = [&](Set &r, uint32_t m0) ALWAYS_INLINE {
-        if (m0 + kGradStep <= plain_to) return plain_k(r, m0);
+    auto request_k = [&](Set &r, int i0, int i1, uint32_t m0) ALWAYS_INLINE {
+        if (m0 + kGradStep <= plain_to) return plain_k(r, i0, i1, m0);
 #pragma unroll
-        for (int i = 0; i < C::LOAD_K; ++i) {
+        for (int i = i0; i < i1; ++i) {
             const uint32_t m = m0 + row_k + i * ROWS_K;
             const size_t row = m < to ? m : p.rows - 1;
             r.ok[i].request((const char *)p.q + row * p.ldq, ck, p.cols);
@@ -212,9 +213,9 @@ __global__ void __launch_bounds__(C::THREADS) weight_grad_kernel(const WeightGra
 
     if (wave >= C::COMPUTE / 64) {
         // ---- The copying waves.  One pair brings the even steps from registers to LDS, the other the odd ones, each for two turns of the
-        // computing waves, so that one converts while the other's loads are issued.  A step s is written in turns s - 3 (dy) and s - 2 (codes),
-        // and what step s + 2 holds is requested in its place, two turns ahead: of the four buffers, those of s - 3, s - 2 and s - 1
-        // may be read in those turns.  The sums of dy are one more product, with ones.
+        // computing waves, so that one converts while the other's loads are issued.  A step s is written in turns s - 3 and s - 2, and
+        // what step s + 2 holds is requested in its place, two turns ahead (four ahead, in a second set of registers, gained nothing): of the four buffers, those of s - 3, s - 2 and s - 1 may be
+        // read in those turns.  The sums of dy are one more product, with ones.
         const uint32_t w = wave - C::COMPUTE / 64, pair = w >> 1;
         const int one = C::DY == QGEMM_DT_BF16 ? 0x3F803F80 : 0x3C003C00;
         const v4i ones = v4i{one, one, one, one};
@@ -229,60 +230,66 @@ __global__ void __launch_bounds__(C::THREADS) weight_grad_kernel(const WeightGra
                 for (int i = 0; i < C::FS; ++i) sum[i] = multiply(ones, fragment(buffer(t), w * C::FS + i), sum[i]);
             }
         };
-        auto first_half = [&](uint32_t s, auto plain) ALWAYS_INLINE {
+        // Half of a step's octets: half of dy's and half of the codes', or in the smaller tiles dy in the first turn and the codes in the second.  (us,
+        // the second way and then the first: 256 x 256 tiles, 8192 x 8192 x 4096 516 and 492; 128 x 128 tiles, 1999 x 3001 x 1000 35.2 and 36.7.)
+        auto half = [&](Set &r, auto which, uint32_t s, auto plain) ALWAYS_INLINE {
+            constexpr int W = which.value, N0 = C::EVEN ? W * C::LOAD_N / 2 : W * C::LOAD_N, N1 = C::EVEN ? N0 + C::LOAD_N / 2 : C::LOAD_N;
+            constexpr int K0 = C::EVEN ? W * C::LOAD_K / 2 : 0, K1 = C::EVEN ? K0 + C::LOAD_K / 2 : W * C::LOAD_K;
 #pragma unroll
-            for (int i = 0; i < C::LOAD_N; ++i) stage_n(r, i, buffer(s));
+            for (int i = N0; i < N1; ++i) stage_n(r, i, buffer(s));
+#pragma unroll
+            for (int i = K0; i < K1; ++i) stage_k(r, i, buffer(s));
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (plain.value) plain_n(r, from + (s + 2) * kGradStep);
-            else if (s + 2 < steps) request_n(r, from + (s + 2) * kGradStep);
+            if constexpr (plain.value) {
+                plain_n(r, N0, N1, from + (s + 2) * kGradStep);
+                plain_k(r, K0, K1, from + (s + 2) * kGradStep);
+            } else if (s + 2 < steps) {
+                request_n(r, N0, N1, from + (s + 2) * kGradStep);
+                request_k(r, K0, K1, from + (s + 2) * kGradStep);
+            }
             __builtin_amdgcn_sched_barrier(0);
         };
-        auto second_half = [&](uint32_t s, auto plain) ALWAYS_INLINE {
-#pragma unroll
-            for (int i = 0; i < C::LOAD_K; ++i) stage_k(r, i, buffer(s));
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (plain.value) plain_k(r, from + (s + 2) * kGradStep);
-            else if (s + 2 < steps) request_k(r, from + (s + 2) * kGradStep);
-            __builtin_amdgcn_sched_barrier(0);
-        };
+        constexpr std::integral_constant<int, 0> first;
+        constexpr std::integral_constant<int, 1> second;
         // Steps whose requests are plain have no branch around them, nor have those in front of them: behind one the compiler takes the
         // fewest loads that may be in flight on either way, and waits for more than it has to.
         const uint32_t plain_steps = plain_to > from ? (plain_to - from) / kGradStep : 0;
         uint32_t s = pair, turns = steps + 1;             // the step that is written next; barriers still to come
-        auto both = [&](auto plain) ALWAYS_INLINE {
-            first_half(s, plain);
+        auto both = [&](Set &r, auto plain) ALWAYS_INLINE {
+            half(r, first, s, plain);
             add_up(s - 3);                                // (in front of the first turn, s = 2: none)
             __syncthreads();
-            second_half(s, plain);
+            half(r, second, s, plain);
             add_up(s - 2);
             __syncthreads();
             s += 2;
             turns -= 2;
         };
         auto first_step = [&](auto plain) ALWAYS_INLINE {
-            first_half(s, plain);
-            second_half(s, plain);
+            half(r, first, s, plain);
+            half(r, second, s, plain);
             s += 2;
             if (pair == 1) {                              // (the even steps are a turn ahead)
                 __syncthreads();
                 --turns;
             }
         };
-        if (plain_steps >= 6) {
-            plain_n(r, from + s * kGradStep);
-            plain_k(r, from + s * kGradStep);
+        if (plain_steps >= 4) {
+            plain_n(r, 0, C::LOAD_N, from + s * kGradStep);
+            plain_k(r, 0, C::LOAD_K, from + s * kGradStep);
+            __builtin_amdgcn_sched_barrier(0);
             first_step(std::true_type{});
 #pragma unroll 1
-            while (s + 3 <= plain_steps) both(std::true_type{});
+            while (s + 3 <= plain_steps) both(r, std::true_type{});
         } else {
             if (s < steps) {
-                request_n(r, from + s * kGradStep);
-                request_k(r, from + s * kGradStep);
+                request_n(r, 0, C::LOAD_N, from + s * kGradStep);
+                request_k(r, 0, C::LOAD_K, from + s * kGradStep);
             }
             first_step(std::false_type{});
         }
 #pragma unroll 1
-        while (turns >= 2) both(std::false_type{});
+        while (turns >= 2) both(r, std::false_type{});
         if (turns) {
             add_up(s - 3);
             __syncthreads();
@@ -301,33 +308,34 @@ __global__ void __launch_bounds__(C::THREADS) weight_grad_kernel(const WeightGra
         return;
     }
 
-    // ---- The computing waves: products of step t, while the first fragments of step t + 1, which is whole, are on their way
+    // ---- The computing waves: products of step t, while the first fragments of step t + 1, which is whole, are on their way: the codes' go where
+    // the last products of step t let go of theirs.  (All fragments of a step read during the step in front, in tiles with registers for both, changed
+    // no time by more than 2 %.)
     const uint32_t wn = wave / C::WK, wk = wave % C::WK;
     v4f acc[C::FN][C::FK] = {};
-    v4i x[C::FK], y[C::Y];
-    auto first_fragments = [&](const char *of) ALWAYS_INLINE {
-#pragma unroll
-        for (int g = 0; g < C::FK; ++g) x[g] = fragment(of + C::BN / 64 * C::PANEL, wk * C::FK + g);
-#pragma unroll
-        for (int i = 0; i < C::AHEAD; ++i) y[i] = fragment(of, wn * C::FN + i);
-    };
+    auto fragment_x = [&](const char *of, int g) ALWAYS_INLINE { return fragment(of + C::BN / 64 * C::PANEL, wk * C::FK + g); };
+    auto fragment_y = [&](const char *of, int f) ALWAYS_INLINE { return fragment(of, wn * C::FN + f); };
     __syncthreads();
-    first_fragments(lds);
+    v4i x[C::FK], y[C::AHEAD + 1];
+#pragma unroll
+    for (int g = 0; g < C::FK; ++g) x[g] = fragment_x(lds, g);
+#pragma unroll
+    for (int i = 0; i < C::AHEAD; ++i) y[i] = fragment_y(lds, i);
 #pragma unroll 1
     for (uint32_t t = 0; t < steps; ++t) {
         const char *now = buffer(t), *then = buffer(t + 1);
 #pragma unroll
         for (int f = 0; f < C::FN; ++f) {
-            if (f + C::AHEAD < C::FN) y[(f + C::AHEAD) % C::Y] = fragment(now, wn * C::FN + f + C::AHEAD);
+            if (f + C::AHEAD < C::FN) y[(f + C::AHEAD) % (C::AHEAD + 1)] = fragment_y(now, f + C::AHEAD);
 #pragma unroll
             for (int g = 0; g < C::FK; ++g) {
-                acc[f][g] = multiply(x[g], y[f % C::Y], acc[f][g]);
-                if (f == C::FN - 1) x[g] = fragment(then + C::BN / 64 * C::PANEL, wk * C::FK + g);
+                acc[f][g] = multiply(x[g], y[f % (C::AHEAD + 1)], acc[f][g]);
+                if (f == C::FN - 1) x[g] = fragment_x(then, g);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int i = 0; i < C::AHEAD; ++i) y[i] = fragment(then, wn * C::FN + i);
+        for (int i = 0; i < C::AHEAD; ++i) y[i] = fragment_y(then, i);
         __builtin_amdgcn_sched_barrier(0);
         // (nothing of this wave has to arrive anywhere in front of the barrier: the fragments of step t are in its products)
         asm volatile("s_barrier" ::: "memory");
