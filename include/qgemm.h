@@ -252,7 +252,8 @@ int qgemm_quantize_grid(int in_dtype, size_t rows, size_t cols, uint32_t *rows_p
  *   QGEMM_ERR_UNSUPPORTED, a name no family has is QGEMM_ERR_INVALID_ARG here.
  * qgemm_variant_count / qgemm_variant_name enumerate the rows of the family that serves (in_dtype, scale_mode,
  *   k_major) -- arguments as for qgemm_plan -- so that callers never depend on the order of a table.
- * qgemm_last_config writes the name of the kernel variant the last GEMM call chose. */
+ * qgemm_last_config writes the name of the kernel variant the last GEMM call chose ("layer_norm", "layer_norm_backward", "checkpoint",
+ * "restore", "weight_gradient_128x128" / "_256x128" / "_256x256" with "_split<slices>" after those calls). */
 int qgemm_set_option(const char *key, long value);
 int qgemm_force_config(const char *name);
 int qgemm_variant_count(int in_dtype, int scale_mode, int k_major);
