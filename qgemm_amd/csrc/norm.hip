@@ -141,9 +141,12 @@ hipError_t launch_layer_norm_backward(const NormBackwardArgs &a, int cus, hipStr
             return with_any_type(a.x_dt, [&](auto x) {
                 if (in_registers(a.cols))
                     return with_backward_shape(backward_shape(a.cols), [&](auto group, auto p) {
-                        return launch_kernel(a.cols % kOctet ? norm_backward_rows_kernel<dy.value, x.value, group.value, p.value, ROW_RAGGED>
-                                                             : norm_backward_rows_kernel<dy.value, x.value, group.value, p.value, ROW_WHOLE>,
-                                             dim3(row_workgroups(a, cus)), dim3(group.value < 256 ? 256 : group.value), 0, stream, a);
+                        auto kernel = a.cols % kOctet ? norm_backward_rows_kernel<dy.value, x.value, group.value, p.value, ROW_RAGGED>
+                                                      : norm_backward_rows_kernel<dy.value, x.value, group.value, p.value, ROW_WHOLE>;
+                        if constexpr ((x.value == QGEMM_DT_I8 || x.value == QGEMM_DT_F8E4M3) && group.value > 16)      // (two blocks or more)
+                            if (a.cols % kScaleBlock - 1 < kOctet - 1)
+                                kernel = norm_backward_rows_kernel<dy.value, x.value, group.value, p.value, ROW_RAGGED, true>;
+                        return launch_kernel(kernel, dim3(row_workgroups(a, cus)), dim3(group.value < 256 ? 256 : group.value), 0, stream, a);
                     });
                 hipError_t f = launch_kernel(norm_backward_any_kernel<dy.value, x.value>, dim3(std::min(a.rows, kMostRowGroups)), dim3(256), 0, stream, a);
                 if (f == hipSuccess && a.groups)

@@ -15,7 +15,8 @@ using row_offset = std::conditional_t<ROW == ROW_ANY, size_t, uint32_t>;
 // A row that ends inside its last octet: no lane reads behind it, and nothing branches between loads, as the last eight elements are
 // fetched from where they lie.
 //   ROW_RAGGED  the lane works on those eight: the first `repeated` of them are the octet in front's as well, count in no sum and are
-//               written twice, with the same values.  (Moving them down instead, and writing the end element by element, kept one wave of
+//               written twice, with the same values.  (They may lie in the block of 128 columns in front of the lane's own, which has another
+//               scale: whatever comes out of codes there takes the scale of column cols - 8 for them.)  (Moving them down instead, and writing the end element by element, kept one wave of
 //               every row a third longer than the others: norm of 4096 x 3001 bf16 19.1 us, 14.2 for 3000)
 //   ROW_ANY     they are moved down, zeros behind them; rows of fewer than eight are fetched one by one
 template <int ROW>
