@@ -381,7 +381,8 @@ __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) norm_backward_rows_
             r.dy[i].hold();
             r.x[i].o.hold();
             r.dy[i].floats(g);
-            r.x[i].values(r.mean, r.rstd, xhat);
+            // (behind the row's end x - mean is -mean, and its product with rstd may be infinite: 0 times it is no 0)
+            r.x[i].values(r.mean, CODES || column(i) < cols ? r.rstd : 0.0f, xhat);
             if (any_repeated<ROW>(column(i), cols))
 #pragma unroll
                 for (int e = 0; e < 8; ++e) g[e] = e < (int)repeated<ROW>(column(i), cols) ? 0.0f : g[e];
