@@ -193,7 +193,7 @@ int qgemm_layer_norm(int x_dtype, int y_dtype, int param_dtype, int q_dtype, con
  *   dx = rstd * (g - sum(g) / cols - xhat * sum(g * xhat) / cols), dweight = sum over rows of dy * xhat, dbias = sum over rows of dy
  *   x        the norm's input (mean is needed then), or xhat in 8 bits: x_dtype I8 / F8E4M3 with its scales (mean is ignored)
  *   dweight, dbias  cols elements of param_dtype each, overwritten; NULL where nobody wants them.  Partial sums go through the
- *            library workspace */
+ *            library workspace.  (Up to 2^31 - 128 columns) */
 int qgemm_layer_norm_backward(int dy_dtype, int x_dtype, int dx_dtype, int param_dtype, const void *dy, size_t lddy, const void *x, size_t ldx,
                               const float *scales, const float *mean, const float *rstd, const void *weight, void *dx, size_t lddx,
                               void *dweight, void *dbias, size_t rows, size_t cols, void *stream);

@@ -7,6 +7,7 @@ namespace qgemm {
 
 namespace {
 constexpr uint32_t kMostRowGroups = 1 << 16;          // workgroups that share out the rows of a launch
+constexpr uint32_t kMostColumnGroups = 1 << 16;       // workgroups across of the parameters' sums: a launch has fewer than 2^32 threads across
 
 template <class F>
 auto with_type(int dt, F f) {
@@ -155,8 +156,10 @@ hipError_t launch_layer_norm_backward(const NormBackwardArgs &a, int cus, hipStr
             });
         });
     }
-    if (e == hipSuccess && (a.dweight || a.dbias))
-        e = launch_kernel(norm_parameter_sums_kernel, dim3((a.cols + 31) / 32, 2), dim3(512), 0, stream, a);
+    if (e == hipSuccess && (a.dweight || a.dbias)) {
+        const uint32_t groups = (a.cols + 31) / 32, across = std::min(groups, kMostColumnGroups);
+        e = launch_kernel(norm_parameter_sums_kernel, dim3(across, (groups + across - 1) / across * 2), dim3(512), 0, stream, a);
+    }
     return e;
 }
 

@@ -527,15 +527,16 @@ __global__ void __launch_bounds__(256) norm_column_sums_kernel(const NormBackwar
 }
 
 // dweight / dbias out of the workgroups' sums: 32 columns a workgroup, 64 partial sums at a time, eight of which a lane has in flight, always in
-// the same order.  blockIdx.y: which of the two.  512 rows of 4096 columns 4.5 us, three trips to memory one behind the other.
+// the same order.  blockIdx.y: which of the two, and the columns that x, of kMostColumnGroups workgroups at the most, leaves over.  512 rows of
+// 4096 columns 4.5 us, three trips to memory one behind the other.
 __global__ void __launch_bounds__(512) norm_parameter_sums_kernel(const NormBackwardArgs p) {
     constexpr uint32_t SLICES = 64, DEEP = 8;
     __shared__ v4f red[SLICES][8];
     const size_t stride = norm_partial_cols(p.cols);
-    const uint32_t lane = threadIdx.x & 7, sub = threadIdx.x >> 3, which = blockIdx.y;
+    const uint32_t lane = threadIdx.x & 7, sub = threadIdx.x >> 3, which = blockIdx.y & 1, c0 = ((blockIdx.y >> 1) * gridDim.x + blockIdx.x) * 32;
     void *out = which ? p.dbias : p.dweight;
-    if (!out) return;
-    const float *in = p.partial + which * stride + (size_t)blockIdx.x * 32 + lane * 4;
+    if (!out || c0 >= p.cols) return;
+    const float *in = p.partial + which * stride + c0 + lane * 4;
     v4f s = v4f{0, 0, 0, 0};
     for (uint32_t g = sub; g < p.groups; g += SLICES * DEEP) {
         v4f v[DEEP];
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(512) norm_parameter_sums_kernel(const NormBack
         if (sub < half) red[sub][lane] += red[sub + half][lane];
         __syncthreads();
     }
-    const uint32_t c = blockIdx.x * 32 + threadIdx.x;
+    const uint32_t c = c0 + threadIdx.x;
     if (threadIdx.x >= 32 || c >= p.cols) return;
     const float *at = (const float *)red + threadIdx.x;
     float v = at[0];

@@ -2125,6 +2125,7 @@ QGEMM_EXPORT int qgemm_layer_norm_backward(int dy_dtype, int x_dtype, int dx_dty
     if ((weight || dweight || dbias) && !is_float_type(param_dtype)) return QGEMM_ERR_UNSUPPORTED;
     if (cols == 0) return QGEMM_ERR_INVALID_ARG;
     if (rows >= ((size_t)1 << 31) || cols >= ((size_t)1 << 31)) return QGEMM_ERR_TOO_LARGE;
+    if ((dweight || dbias) && cols > ((size_t)1 << 31) - 128) return QGEMM_ERR_TOO_LARGE;      // (2^32 threads of the columns' sums)
     if (rows && (!dy || !x || !dx || !rstd || (codes ? !scales : !mean) || lddy < cols || ldx < cols || lddx < cols)) return QGEMM_ERR_INVALID_ARG;
     if (rows == 0 && !dweight && !dbias) return QGEMM_OK;
     hipStream_t stream = (hipStream_t)stream_;
