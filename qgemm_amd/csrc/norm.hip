@@ -7,6 +7,7 @@ namespace qgemm {
 
 namespace {
 constexpr uint32_t kMostRowGroups = 1 << 16;          // workgroups that share out the rows of a launch
+constexpr size_t kMostPartials = (size_t)128 << 20;   // partial sums that a stream's own workspace block holds (registers' forms need 32 MiB at the most)
 constexpr uint32_t kMostColumnGroups = 1 << 16;       // workgroups across of the parameters' sums: a launch has fewer than 2^32 threads across
 
 template <class F>
@@ -132,7 +133,9 @@ uint32_t row_workgroups(const NormBackwardArgs &a, int cus) {
 
 uint32_t norm_backward_groups(const NormBackwardArgs &a, int cus) {
     if (a.rows == 0 || (!a.dweight && !a.dbias)) return 0;
-    return in_registers(a.cols) ? row_workgroups(a, cus) : std::min<uint32_t>((a.rows + 15) / 16, 64);
+    if (in_registers(a.cols)) return row_workgroups(a, cus);
+    const size_t room = std::max<size_t>(kMostPartials / norm_partial_bytes(1, a.cols), 1);
+    return (uint32_t)std::min<size_t>({(a.rows + 15) / 16, 64, room});
 }
 
 hipError_t launch_layer_norm_backward(const NormBackwardArgs &a, int cus, hipStream_t stream) {

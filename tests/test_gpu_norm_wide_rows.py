@@ -9,7 +9,7 @@ from tests.util import say
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("rows,cols", [(3, (1 << 21) + 37), (2, (1 << 22) - 1), (1, (1 << 28) + 5)])
+@pytest.mark.parametrize("rows,cols", [(3, (1 << 21) + 37), (2, (1 << 22) - 1), (1, (1 << 28) + 5), (600, (1 << 20) + 9)])
 def test_sums_of_every_column(rows, cols):
     say("layer_norm_backward wide rows", rows, cols)
     g = torch.Generator(device="cuda").manual_seed(cols)
@@ -18,7 +18,7 @@ def test_sums_of_every_column(rows, cols):
     dx, dw, db = Q.layer_norm_backward(dy, x, mean, rstd, w, out_dtype=torch.float32)
     # (whole numbers: the columns' sums are exact)
     assert torch.equal(db, dy.float().sum(0)) and torch.equal(dw, (dy.float() * x.float()).sum(0))
-    for row in range(rows):
+    for row in range(0, rows, max(1, rows // 3)):
         d, v = dy[row].double(), x[row].double()
         a, b = d.mean(), (d * v).mean()
         # a lane adds up every 256th octet, one after the other

@@ -57,3 +57,27 @@ for _ in range(3000):
     check(("gradient", rows, n, cols), gradient(rows, n, cols))
 assert backward(3, 1 << 28) == OK and backward(0, (1 << 31) - 128) == OK
 """)
+
+
+def test_partial_sums_stay_within_their_room(host):
+    """Sums of columns that pass through the workspace: 128 MiB at the most, or the eight bytes a column that one part of them takes."""
+    host("""
+import random
+rng = random.Random(2)
+runtime.host_budget(1 << 62)
+def most():
+    sizes = [int(e.split()[1]) for e in events() if e.startswith("malloc")]
+    return max(sizes, default=0)
+for rows, cols in [(1009, 1 << 18), (5000, (1 << 18) + 1), (70000, 1 << 20), (1 << 20, 16384), (16, 1 << 24), (17, 1 << 24), (3000, 1 << 28)] + \
+                  [(int(2 ** rng.uniform(0, 20)), int(2 ** rng.uniform(0, 28))) for _ in range(500)]:
+    lib.qgemm_shutdown()
+    events()
+    assert backward(rows, cols) == OK
+    took = most()
+    assert took <= max(128 << 20, 8 * ((cols + 63) // 64 * 64)), (rows, cols, took)
+    lib.qgemm_shutdown()
+    events()
+    assert backward(rows, cols, dweight=None) == OK and most() == 0
+    n, cols = int(2 ** rng.uniform(0, 14)), int(2 ** rng.uniform(0, 14))
+    assert gradient(rows, n, cols) == OK and most() <= 128 << 20, (rows, n, cols)
+""")
