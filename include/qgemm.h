@@ -175,7 +175,8 @@ int qgemm_quantize(int in_dtype, int out_dtype, int mode, const void *x, size_t 
  * scales[row * ceil(cols / 128) + col / 128], the arrangement of QGEMM_QUANT_BLOCK_1x128 with K-contiguous scales; it stands for q * scale.
  * What the entries below write has powers of two as scales: s is the smallest (2^-126 at the least) with max|v| <= 127 s (448 s), 1
  * for a block of zeros, q = rne(v / s); at the top of the type's range codes stop where q * s would be infinite.  q * s is then exact in
- * bf16 (and in fp16 down to its smallest numbers).  A block with an infinity or NaN gets s = NaN and reads as NaN throughout.  What the
+ * bf16 (F8E4M3: from s = 2^-124 on, below a bf16 multiple of 2^-133), and in fp16 where it is at most 65504 and s is 2^-24 (F8E4M3: 2^-15) or more,
+ * below a multiple of 2^-24.  A block with an infinity or NaN gets s = NaN and reads as NaN throughout.  What the
  * entries below read may have any scales, those of qgemm_quantize among them.
  *
  * Types are F32, BF16 or F16 unless said otherwise; leading dimensions count elements.  Zero rows are no error: gradients
@@ -198,7 +199,8 @@ int qgemm_layer_norm_backward(int dy_dtype, int x_dtype, int dx_dtype, int param
                               const float *scales, const float *mean, const float *rstd, const void *weight, void *dx, size_t lddx,
                               void *dweight, void *dbias, size_t rows, size_t cols, void *stream);
 
-/* An activation into 8 bits, and back (x = q * scale, rounded once where x_dtype has fewer bits). */
+/* An activation into 8 bits, and back: x = q * scale, a product of fp32, rounded to x_dtype.  (Under scales that are no powers of two
+ * the fp32 product is rounded already.) */
 int qgemm_checkpoint(int x_dtype, int q_dtype, const void *x, size_t ldx, size_t rows, size_t cols, void *q, size_t ldq, float *scales,
                      void *stream);
 int qgemm_restore(int q_dtype, int x_dtype, const void *q, size_t ldq, const float *scales, size_t rows, size_t cols, void *x, size_t ldx,
@@ -206,8 +208,8 @@ int qgemm_restore(int q_dtype, int x_dtype, const void *q, size_t ldq, const flo
 
 /* Gradients of a linear layer z = v W^T + c out of its input v in 8 bits:
  *   dw[n x cols] = dy^T v and db[n] = sum over rows of dy
- *   dy       rows x n, BF16 or F16: v is widened to that type in front of the matrix cores (exact where scales are powers of two;
- *            F16: beyond 65504 infinite)
+ *   dy       rows x n, BF16 or F16: v is widened to that type in front of the matrix cores (exact where q * scale is, see above; else
+ *            the fp32 product is rounded to it; F16: beyond 65504 infinite)
  *   weight, bias  cols elements of param_dtype each, or NULL: q holds a layer norm's xhat and v = xhat * weight + bias is meant
  *   dw       of dw_dtype, overwritten; fp32 accumulation.  Few tiles of it split the rows between workgroups through the library workspace
  *   db       n floats, or NULL */

@@ -219,7 +219,8 @@ __device__ __forceinline__ uint32_t block_max_bits(const float (&v)[8]) {
 // ---- 8-bit codes under a scale that is a power of two
 // s is the smallest power of two (2^-126 at the least) with max|v| <= 127 s (int8) or 448 s (e4m3), 1 for zeros; q = rne(v / s), and v / s is
 // exact.  Powers of two cost up to one bit of the eight against s = max / 127, and buy that q s needs no more bits than q: it is
-// exact in bf16 and, down to its smallest numbers, in fp16, so that a product that reads q s on the 16-bit matrix cores rounds nothing.
+// exact in bf16, and in fp16 within its range, so that a product that reads q s on the 16-bit matrix cores rounds nothing.  (Where q s is no multiple of
+// the type's smallest number it is rounded to one: bf16 from e4m3 under s < 2^-124, fp16 under s < 2^-24, from e4m3 under s < 2^-15.)
 // A block with an infinity or a NaN gets s = NaN: all of it reads as NaN, and nothing is hidden from what is computed from it.
 struct PowerOfTwo {
     float s, inv;       // the scale and 1 / s; inv is 0 where s is NaN

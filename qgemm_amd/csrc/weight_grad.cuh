@@ -3,8 +3,9 @@
 // was xhat w + b, the two vectors leave the sum: dW[n, k] = w[k] sum dy xhat + b[k] db[n], and the product reads codes alone.
 //
 // Both operands lie with their rows along the contraction, as they were written.  A step is 32 rows: dy goes from memory through registers
-// into LDS as it is, codes are widened to dy's type on the way (exact where scales are powers of two: the only rounding there is otherwise), and
-// the matrix cores' operands, which run along the rows, are taken out of both with transposing reads.  fp32 accumulators, fp32 planes.
+// into LDS as it is, codes are widened to dy's type on the way (exact for powers of two as scales, see power_of_two; other scales' products are
+// rounded to fp32 and then to dy's type), and the matrix cores' operands, which run along the rows, are taken out of both with transposing reads.
+// fp32 accumulators, fp32 planes.
 //
 // What bounds it: at 8192 x 8192 x 4096 (bf16, int8 codes) 480 - 510 us, 1.08 - 1.14 PFLOP/s of the 1.54 that the product of two bf16 matrices
 // reaches at 8192^3 on the same card.  Steps to there, us: waves that load, convert and multiply in turn, 128 x 128 tiles 1118, 256 x 256 610;

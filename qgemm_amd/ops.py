@@ -410,7 +410,8 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, scales=None, bias=True, 
 
 def checkpoint(x, dtype=torch.int8):
     """q, scales = an activation x [..., cols], fp32 / bf16 / fp16, in 8 bits for the backward pass: codes (torch.int8 or torch.float8_e4m3fn) and
-    one power of two for the 128 columns of a block, scales [..., ceil(cols/128)].  q * scale is exact in bf16."""
+    one power of two for the 128 columns of a block, scales [..., ceil(cols/128)].  q * scale is exact in bf16
+    (float8_e4m3fn: under scales of 2^-124 and more)."""
     native = _native()
     if native:
         st, q, scales = native.ops_checkpoint(x, dtype)
