@@ -45,8 +45,8 @@ hipError_t with_shape(NormShape s, F f) {
     return hipErrorInvalidValue;
 }
 // Up to kFewRows rows, which one round of workgroups holds, more threads for a row end it sooner; beyond it fewer threads of more octets leave
-// room for more rows (us, 6144 x 7168 bf16 kept: 256 threads of four 43.3, 512 of two 51.4; 128 x 8192 5.4 and 4.9; 16384 x 2048: 64 of four 30.6,
-// 256 of one 39.4, 1 x 2048 4.1 and 3.1).
+// room for more rows (us, 6144 x 7168 bf16 kept: 256 threads of four 42.5, 512 of two 50.0, on other buffers each time 54.5 and 58.0, not kept 35.0
+// and 43.8; 128 x 8192 5.4 and 4.9; 16384 x 2048: 64 of four 30.6, 256 of one 39.4, 1 x 2048 4.1 and 3.1).
 constexpr uint32_t kFewRows = 1024, kMostCols = 16384;
 bool in_registers(uint32_t cols) { return cols >= kOctet && cols <= kMostCols; }
 NormShape norm_shape(uint32_t rows, uint32_t cols) {

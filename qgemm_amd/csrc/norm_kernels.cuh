@@ -66,7 +66,9 @@ __device__ __forceinline__ void affine(const NormArgs &p, uint32_t c, const floa
 }
 
 // ---- rows of any length: a workgroup goes over its row three times, the second and third time out of the caches.  Rows that the registers of
-// 512 threads do not hold, or of a few elements; 8192 x 20000 bf16 218 us, 3.0 TB/s, bound by the trips to the caches.
+// 512 threads do not hold, or of a few elements; 8192 x 20000 bf16 218 us, 3.0 TB/s, bound by the trips to the caches.  And parameters whose type is
+// neither x's nor fp32, at any width (us, parameters of x's type or fp32 / of another: 4096 x 7168 fp32 with bf16 42 / 63, bf16 with fp16 26 / 36,
+// 1 x 7168 4.1 / 7.2; on short rows most of the 256 threads have nothing to do: 131072 x 128 bf16 with fp16 14 / 184).
 template <int DT>
 __global__ void __launch_bounds__(256) norm_any_kernel(const NormArgs p) {
     __shared__ float red[2][4][1];
@@ -127,7 +129,8 @@ __global__ void __launch_bounds__(256) norm_any_kernel(const NormArgs p) {
 // once: with n_w elements, mean m_w and squares M_w of part w, sum (x - mean)^2 = sum M_w + n_w (m_w - mean)^2, which cancels nothing.
 // SAME: the parameters have x's type, else they are fp32.  AHEAD: an octet of them is requested in front of the one that is being worked
 // on, the first with the row: half a trip to memory less for a row by itself, and registers that many rows want for more waves
-// (us, without / with: 1 x 7168 bf16 4.3 / 3.9, 6144 x 7168 43.3 / 49.8).  ROW: see RowKind.
+// (us, without / with: 1 x 7168 bf16 4.3 / 3.9, 6144 x 7168 kept 42.5 / 49.5 on the same buffers again and 54.5 / 62.5 on others each time, not kept
+// 35.0 / 34.5; not all of them: 16384 x 2048 26.0 / 24.1).  ROW: see RowKind.
 template <int DT, int GROUP, int P, bool SAME, bool AHEAD, int ROW>
 __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) norm_rows_kernel(const NormArgs p) {
     constexpr int THREADS = GROUP < 256 ? 256 : GROUP, ROWS = THREADS / GROUP, WAVES = GROUP / 64, LANES = GROUP < 64 ? GROUP : 64;
@@ -324,8 +327,9 @@ __global__ void __launch_bounds__(256) norm_backward_any_kernel(const NormBackwa
 
 // Rows in registers: GROUP threads hold a row of dy and of x, P octets each; a workgroup goes over its rows with the next one's
 // loads in flight, and keeps the sums of its columns in registers until the end: dy and x are read once.  Bound by memory: 8192 x 4096 bf16 36 us,
-// 5.7 TB/s, and 4.5 for the workgroups' sums; with a second reading for the columns it was 76.  1999 x 3001 fp16 out of e4m3 12.7, 2.4 TB/s: eight
-// rows a workgroup, each at an odd address, and one in flight.
+// 5.7 TB/s, and 4.5 for the workgroups' sums; with a second reading for the columns it was 76.  1999 x 3001 fp16 out of e4m3 14.4, 2.1 TB/s: eight
+// rows a workgroup, each at an odd address, and one in flight.  Four octets (8193 - 16384 columns) are more than the registers hold beside the next
+// row: 12 - 320 bytes a lane in scratch; 4096 x 14336 bf16 79 us with the sums' launch, 69 at the rate of a copy.
 // EDGE: out of codes, rows that end one to seven columns into a block of 128.  What their last octet repeats lies under the scale of the block in
 // front, and dx is the same from both lanes that write it only where both take that one.  A form of its own, because the scale in flight costs
 // other ragged rows 2 - 9 % (us, without / with: 1999 x 3001 fp16 out of e4m3 17.4 / 18.3, 4096 x 8237 bf16 out of int8 57.2 / 62.8; loaded where
