@@ -217,6 +217,76 @@ int qgemm_weight_gradient(int dy_dtype, int q_dtype, int dw_dtype, int param_dty
                           const float *scales, const void *weight, const void *bias, void *dw, size_t lddw, float *db, size_t rows,
                           size_t n, size_t cols, void *stream);
 
+/* ---- Beside the products of a language model (no counterpart in the reference): the root-mean-square norm in front of them, low-rank adapters
+ * added to their results, log probabilities out of the last one.  Types are F32, BF16 or F16 unless said otherwise; leading dimensions count
+ * elements.  All sums are fp32, in an order that is the same from run to run.  Outputs must not overlap inputs unless said otherwise. */
+
+/* h = x + residual, rounded to residual_dtype; rstd = 1 / sqrt(sum h^2 / cols + eps) of what is stored; y = h * rstd * weight.
+ *   residual, h   rows x cols of residual_dtype, or both NULL: h is x
+ *   weight        cols elements of param_dtype, or NULL: 1
+ *   y, q          y in y_dtype, and in 8 bits (q_dtype I8 or F8E4M3): s = max|y| / 127 (448) of a row's 128 columns, scales[row * ceil(cols / 128) + col / 128],
+ *                 q = rne(y / s) of the fp32 y, 1 for zeros: the operand of QGEMM_SCALE_BLOCK128 products; a block with an infinity or NaN gets
+ *                 s = NaN.  One of the two may be NULL (q with scales)
+ *   rstd          rows floats for the backward pass, or NULL
+ * (Squares are summed in fp32: rows beyond 1e19 / sqrt(cols) in magnitude overflow, and give rstd = 0.) */
+int qgemm_rms_norm(int x_dtype, int residual_dtype, int y_dtype, int param_dtype, int q_dtype, const void *x, size_t ldx, const void *residual,
+                   size_t ldr, const void *weight, float eps, void *h, size_t ldh, void *y, size_t ldy, float *rstd, void *q, size_t ldq,
+                   float *scales, size_t rows, size_t cols, void *stream);
+
+/* Backward pass of qgemm_rms_norm: with g = dy * weight, xhat = h * rstd
+ *   dx = rstd * (g - xhat * sum(g * xhat) / cols) + dh, dweight = sum over rows of dy * xhat
+ *   dh        what arrives along the residual stream, or NULL; dx is then the gradient of x and of the residual
+ *   dweight   cols elements of param_dtype, overwritten (zeros without rows), or NULL.  Partial sums go through the library workspace.  (Up to
+ *             2^31 - 128 columns) */
+int qgemm_rms_norm_backward(int dy_dtype, int h_dtype, int dh_dtype, int dx_dtype, int param_dtype, const void *dy, size_t lddy, const void *h,
+                            size_t ldh, const float *rstd, const void *weight, const void *dh, size_t lddh, void *dx, size_t lddx,
+                            void *dweight, size_t rows, size_t cols, void *stream);
+
+/* Rows grouped by the adapter that each of them has, once for all calls below with the same ids.
+ *   ids      rows integers of id_bytes 4 or 8: 0 .. adapters - 1; any other number means no adapter
+ *   groups   device memory of qgemm_group_rows_words 32-bit words, 8-byte aligned; its contents are the library's own
+ * Up to 65535 adapters and 2^28 - 1 rows. */
+int qgemm_group_rows_words(size_t rows, size_t adapters, size_t *words);
+int qgemm_group_rows(int id_bytes, const void *ids, size_t rows, size_t adapters, void *groups, void *stream);
+
+/* out[t] = y[t] + scaling[i] * B[i]^T (A[i] x[t]) for a row t of adapter i; out[t] = y[t] for a row of none.
+ *   x         rows x k, BF16 or F16 (dtype), as A [adapters x rank x k] and B [adapters x rank x n]: the rank is the rows of both.  Rank up to 128; adapters of
+ *             a lower rank have rows of zeros
+ *   y, out    rows x n of y_dtype; out may be y itself
+ *   scaling   adapters floats, or NULL: 1
+ *   groups    of these rows and this number of adapters
+ *   u         A[i] x[t] for the backward pass, rows x rank floats (zeros for rows of no adapter), or NULL
+ * A[i] x[t] has fp32 accumulators and goes on in 16 bits of mantissa, in 24 where y is F32.  Uses the library workspace.  Up to 2^24 - 256 columns. */
+int qgemm_add_adapters(int dtype, int y_dtype, const void *y, size_t ldy, const void *x, size_t ldx, const void *A, const void *B,
+                       const float *scaling, const void *groups, void *out, size_t ldo, float *u, size_t rows, size_t adapters,
+                       size_t rank, size_t k, size_t n, void *stream);
+
+/* Backward pass of qgemm_add_adapters: v[t] = B[i] dy[t],
+ *   dx[t] = dx0[t] + scaling[i] * A[i]^T v[t], dA[i] = scaling[i] * sum over its rows of v[t] x[t]^T, dB[i] = scaling[i] * sum over its rows of u[t] dy[t]^T
+ *   dy        rows x n of dtype
+ *   dx0, dx   rows x k of dx_dtype: what arrives from the product beside the adapters, NULL: zeros; dx may be dx0 itself, dx NULL: not wanted
+ *   dA, dB    of grad_dtype, overwritten (zeros for an adapter without rows); NULL: not wanted (u is needed for dB only) */
+int qgemm_add_adapters_backward(int dtype, int dx_dtype, int grad_dtype, const void *dy, size_t lddy, const void *x, size_t ldx, const float *u,
+                                const void *A, const void *B, const float *scaling, const void *groups, const void *dx0, size_t lddx0,
+                                void *dx, size_t lddx, void *dA, void *dB, size_t rows, size_t adapters, size_t rank, size_t k, size_t n,
+                                void *stream);
+
+/* For each row of logits, with p = softmax of it: logp = log p[token], entropy = -sum p log p, lse = log sum exp, and the `top` most probable columns:
+ * values log p, indices, equal ones in the order of their columns.
+ *   tokens    rows integers of token_bytes 4 or 8; one outside 0 .. cols - 1 asks for nothing, and its logp is 0
+ *   top       0 .. 32, at most cols; values and indices [rows x top]
+ * -infinity is a column that cannot be.  A row of nothing else has lse = logp = -infinity and entropy 0; one with an infinity or a NaN gives NaNs
+ * (its indices are those of its numbers, NaN counting as -infinity).  Uses the library workspace where rows are few. */
+int qgemm_log_probabilities(int dtype, int token_bytes, const void *logits, size_t ld, const void *tokens, int top, float *logp, float *entropy,
+                            float *lse, float *values, int64_t *indices, size_t rows, size_t cols, void *stream);
+
+/* Backward pass: dlogits_j = dlogp * ([j = token] - p_j) - dentropy * p_j * (log p_j + entropy), of out_dtype
+ *   lse, entropy  as qgemm_log_probabilities gave them; dentropy NULL: zeros (entropy may be NULL then)
+ * A row of nothing but -infinity has the gradient 0, and so has the logp of a row whose token asks for nothing. */
+int qgemm_log_probabilities_backward(int dtype, int out_dtype, int token_bytes, const void *logits, size_t ld, const void *tokens, const float *lse,
+                                     const float *entropy, const float *dlogp, const float *dentropy, void *dlogits, size_t ldd, size_t rows,
+                                     size_t cols, void *stream);
+
 /* Tile raster used by the GEMM kernels: linear workgroup id -> (tile_m, tile_n).
  * Replaces the GROUP_SIZE_M swizzle of src/gemm/sm89_gemm_kernel_v3.cu:169-183
  * (and fixes its clamp), composed with the 8-XCD remap the reference only names
@@ -255,7 +325,8 @@ int qgemm_quantize_grid(int in_dtype, size_t rows, size_t cols, uint32_t *rows_p
  * qgemm_variant_count / qgemm_variant_name enumerate the rows of the family that serves (in_dtype, scale_mode,
  *   k_major) -- arguments as for qgemm_plan -- so that callers never depend on the order of a table.
  * qgemm_last_config writes the name of the kernel variant the last GEMM call chose ("layer_norm", "layer_norm_backward", "checkpoint",
- * "restore", "weight_gradient_128x128" / "_256x128" / "_256x256" with "_split<slices>" after those calls). */
+ * "restore", "weight_gradient_128x128" / "_256x128" / "_256x256" with "_split<slices>", "rms_norm", "rms_norm_backward", "group_rows", "add_adapters",
+ * "add_adapters_backward", "log_probabilities", "log_probabilities_backward" after those calls). */
 int qgemm_set_option(const char *key, long value);
 int qgemm_force_config(const char *name);
 int qgemm_variant_count(int in_dtype, int scale_mode, int k_major);

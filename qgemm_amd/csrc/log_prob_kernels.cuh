@@ -1,0 +1,332 @@
+// Log probabilities of given tokens out of logits, row by row: with m = max x, e = exp(x - m), S = sum e, T = sum e (x - m),
+//   lse = m + log S,   log p of a token = x[token] - lse,   entropy = log S - T / S,   and the largest x with x - lse;
+// and backward, with p = exp(x - lse), a = dlogp, b = dentropy:
+//   dx_j = a ([j = token] - p_j) - b p_j (log p_j + entropy).
+// One pass: every thread keeps the maximum of what it has seen, S and T under it, and puts them right when the maximum grows.  All fp32.
+//
+// Minus infinity is a token that cannot be: p = 0, and it adds nothing to S, T or the gradient.  A row that holds nothing else has lse = -inf,
+// log p = -inf, entropy 0 and gradient 0.  Infinity and NaN make S NaN, and with it all that the row gives.
+//
+// The top k without sorting: L, the k-th largest of 64 groups' maxima, is no more than the k-th largest element, and only threads whose own maximum
+// reaches L hold any element that does.  Their columns are read once more, what reaches L is gathered, and an element's place is the
+// number of those above it.  Elements are compared as 64-bit keys, value above, then the lower index: no two are equal, and the order is that of
+// the values with ties to the lowest index.
+#pragma once
+#include "model.h"
+#include "octet.cuh"
+
+namespace qgemm {
+
+constexpr float kLog2E = 1.44269504088896340736f;
+constexpr float kNothing = -200.0f;                    // exp of it is 0 in fp32, and products with it are finite
+constexpr float kMinusInf = -__builtin_inff();
+
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2E); }
+// S and T from one maximum to a larger one (m = -inf: nothing has been added)
+struct Sums {
+    float m, s, t;
+    __device__ __forceinline__ void raise(float to) {
+        const float d = __builtin_fmaxf(m - to, kNothing), f = m == kMinusInf ? 0.0f : exp_of(d);
+        t = m == kMinusInf ? 0.0f : f * (t + s * d);       // (s and t may be NaN where m is -inf: NaNs alone)
+        s = m == kMinusInf && s == 0.0f ? 0.0f : s * f;
+        m = to;
+    }
+    __device__ __forceinline__ void add(const float (&v)[8], float most) {
+        if (__any(most > m)) raise(__builtin_fmaxf(m, most));
+        const float r = m == kMinusInf ? 0.0f : m;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float d = v[e] - r, w = exp_of(d);
+            s += w;
+            t = __builtin_fmaf(w, __builtin_fmaxf(d, kNothing), t);
+        }
+    }
+};
+__device__ __forceinline__ float max8(const float (&v)[8]) {
+    return __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(v[0], v[1]), __builtin_fmaxf(v[2], v[3])),
+                           __builtin_fmaxf(__builtin_fmaxf(v[4], v[5]), __builtin_fmaxf(v[6], v[7])));
+}
+__device__ __forceinline__ float wave_max(float v) {
+    auto dpp = [&](auto ctrl) {
+        v = __builtin_fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, 0xF, 0xF, true)));
+    };
+    dpp(std::integral_constant<int, 0xB1>{});
+    dpp(std::integral_constant<int, 0x4E>{});
+    dpp(std::integral_constant<int, 0x141>{});
+    dpp(std::integral_constant<int, 0x140>{});
+    uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t a0 = a[0], a1 = a[1];
+    v = __builtin_fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+    u = __builtin_bit_cast(uint32_t, v);
+    const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t b0 = b[0], b1 = b[1];
+    return __builtin_fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+
+// ---- keys: 0 is below every element's
+__device__ __forceinline__ uint32_t order_of(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v != v ? kMinusInf : v + 0.0f);      // (NaN below all numbers; -0 is 0)
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t index) { return (uint64_t)order_of(v) << 32 | (0xFFFFFFFFu - index); }
+__device__ __forceinline__ float value_of(uint64_t key) {
+    const uint32_t o = (uint32_t)(key >> 32);
+    return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+}
+__device__ __forceinline__ uint32_t index_of(uint64_t key) { return 0xFFFFFFFFu - (uint32_t)key; }
+template <int CTRL>
+__device__ __forceinline__ uint64_t key_dpp(uint64_t k) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)k, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(k >> 32), CTRL, 0xF, 0xF, true);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t key_lane(uint64_t k, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(k >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, lane);
+}
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+__device__ __forceinline__ int64_t token_at(const void *tokens, int bytes, uint32_t row) {
+    return bytes == 8 ? ((const int64_t *)tokens)[row] : (int64_t)((const int32_t *)tokens)[row];
+}
+__device__ __forceinline__ float logit_at(const void *row, int dt, size_t c) {
+    if (dt == QGEMM_DT_F32) return ((const float *)row)[c];
+    const uint16_t h = ((const uint16_t *)row)[c];
+    return dt == QGEMM_DT_BF16 ? __builtin_bit_cast(float, (uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
+}
+// a row's numbers out of its sums
+__device__ __forceinline__ float log_prob_finish(const LogProbArgs &p, uint32_t row, float m, float s, float t) {
+    const bool none = s == 0.0f;
+    const float l = logf(s), lse = none ? kMinusInf : m + l;
+    const int64_t token = token_at(p.tokens, p.token_bytes, row);
+    float lp = 0.0f;
+    if (token >= 0 && token < (int64_t)p.cols) {
+        const float x = logit_at((const char *)p.logits + (size_t)row * p.ld * dtype_bytes(p.dt), p.dt, (size_t)token);
+        lp = none ? kMinusInf : x - lse;
+    }
+    p.logp[row] = lp;
+    p.entropy[row] = none ? 0.0f : l - t / s;
+    p.lse[row] = lse;
+    return lse;
+}
+__device__ __forceinline__ void store_top(const LogProbArgs &p, uint32_t row, uint32_t place, uint64_t key, float lse) {
+    const float v = value_of(key);
+    p.values[(size_t)row * p.top + place] = v == kMinusInf && lse == lse ? v : v - lse;
+    p.indices[(size_t)row * p.top + place] = index_of(key);
+}
+
+constexpr uint32_t kLogProbThreads = 256, kLogProbTurn = kLogProbThreads * kOctet, kCandidates = 2048;
+
+// The `top` largest of columns begin .. end - 1, `own` the key of a thread's largest octet (its value, its first column; 0: it has none), to
+// put(place, key) in place 0 .. top - 1, key 0 where there are fewer
+template <int DT, class Put>
+__device__ __forceinline__ void top_of(const void *row, uint32_t begin, uint32_t end, uint32_t top, uint64_t own, Put put) {
+    __shared__ uint64_t group[64], list[kCandidates];
+    __shared__ uint32_t count, holders, holder[kLogProbThreads];
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const uint64_t two = larger(own, key_dpp<0xB1>(own)), four = larger(two, key_dpp<0x4E>(two));
+    if ((tid & 3) == 0) group[tid >> 2] = four;
+    if (tid == 0) count = holders = 0;
+    __syncthreads();
+    uint64_t least = 0;                                    // L
+    {
+        const uint64_t mine = group[lane];
+        uint32_t above = 0;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) above += key_lane(mine, i) > mine ? 1 : 0;
+        const uint64_t at = __ballot(above == top - 1 && mine != 0);
+        if (at) least = key_lane(mine, __builtin_ctzll(at));
+    }
+    // an octet's key stands for any of its elements
+    uint64_t bound = least == 0 ? 0 : (least & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (index_of(least) + kOctet - 1));
+    if (own != 0 && own >= least) holder[atomicAdd(&holders, 1u)] = tid;
+    __syncthreads();
+    const uint32_t turns = (end - begin + kLogProbTurn - 1) / kLogProbTurn, items = holders * turns;
+    for (;;) {
+        for (uint32_t i = tid; i < items; i += kLogProbThreads) {
+            const uint32_t which = i / turns, c = begin + holder[which] * kOctet + (i - which * turns) * kLogProbTurn;
+            if (c >= end) continue;
+            Octet<DT> o;
+            float v[8];
+            o.request(row, c, end);
+            o.settle(c, end);
+            o.floats(v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint64_t key = key_of(v[e], c + e);
+                if (c + e >= end || key < bound) continue;
+                const uint32_t at = atomicAdd(&count, 1u);
+                if (at < kCandidates) list[at] = key;
+            }
+        }
+        __syncthreads();
+        const uint32_t found = count, n = found < kCandidates ? found : kCandidates;
+        __syncthreads();                                   // (count is cleared below)
+        if (found <= kCandidates) {
+            for (uint32_t i = tid; i < n; i += kLogProbThreads) {
+                const uint64_t mine = list[i];
+                uint32_t above = 0;
+                for (uint32_t k = 0; k < n; ++k) above += list[k] > mine ? 1 : 0;
+                if (above < top) put(above, mine);
+            }
+            for (uint32_t i = n + tid; i < top; i += kLogProbThreads) put(i, 0ull);
+            __syncthreads();
+            return;
+        }
+        // more than there is room for: the k-th largest of those that were kept is a higher bound still
+        for (uint32_t i = tid; i < n; i += kLogProbThreads) {
+            const uint64_t mine = list[i];
+            uint32_t above = 0;
+            for (uint32_t k = 0; k < n; ++k) above += list[k] > mine ? 1 : 0;
+            if (above == top - 1) group[0] = mine;
+        }
+        if (tid == 0) count = 0;
+        __syncthreads();
+        bound = group[0];
+        __syncthreads();
+    }
+}
+
+// one workgroup for a split of a row
+template <int DT, bool TOP>
+__global__ void __launch_bounds__(kLogProbThreads) log_prob_kernel(const LogProbArgs p) {
+    constexpr int AHEAD = 4, WAVES = kLogProbThreads / 64;
+    __shared__ float red[3][WAVES];
+    const uint32_t tid = threadIdx.x, begin = blockIdx.x * p.part, end = p.cols - begin < p.part ? p.cols : begin + p.part;
+    for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
+        const char *x = (const char *)p.logits + (size_t)row * p.ld * Octet<DT>::ES;
+        Sums sums{kMinusInf, 0.0f, 0.0f};
+        float best = kMinusInf;
+        uint32_t best_at = begin + tid * kOctet;
+        for (uint32_t c0 = begin + tid * kOctet; c0 < end; c0 += AHEAD * kLogProbTurn) {
+            Octet<DT> o[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) o[i].request(x, c0 + i * kLogProbTurn, end);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const uint32_t c = c0 + i * kLogProbTurn;
+                if (c >= end) break;
+                float v[8];
+                o[i].settle(c, end);
+                o[i].floats(v);
+                if (end - c < kOctet)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = c + e < end ? v[e] : kMinusInf;
+                const float most = max8(v);
+                if (TOP && most > best) {
+                    best = most;
+                    best_at = c;
+                }
+                sums.add(v, most);
+            }
+        }
+        const float wave = wave_max(sums.m);
+        if ((tid & 63) == 0) red[0][tid >> 6] = wave;
+        __syncthreads();
+        float m = red[0][0];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) m = __builtin_fmaxf(m, red[0][i]);
+        sums.raise(m);
+        const float s = lanes_sum<64>(sums.s), t = lanes_sum<64>(sums.t);
+        if ((tid & 63) == 0) {
+            red[1][tid >> 6] = s;
+            red[2][tid >> 6] = t;
+        }
+        __syncthreads();
+        float all_s = red[1][0], all_t = red[2][0];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) {
+            all_s += red[1][i];
+            all_t += red[2][i];
+        }
+        float *part = p.splits > 1 ? p.partial + ((size_t)row * p.splits + blockIdx.x) * log_prob_part(p.top) : nullptr;
+        if (tid == 0) {
+            if (part) {
+                part[0] = m;
+                part[1] = all_s;
+                part[2] = all_t;
+            } else {
+                log_prob_finish(p, row, m, all_s, all_t);
+            }
+        }
+        if constexpr (TOP) {
+            const uint64_t own = begin + tid * kOctet < end ? key_of(best, best_at) : 0;
+            const float lse = all_s == 0.0f ? kMinusInf : m + logf(all_s);
+            top_of<DT>(x, begin, end, p.top, own, [&](uint32_t place, uint64_t key) {
+                if (part) ((uint64_t *)(part + 4))[place] = key;
+                else store_top(p, row, place, key, lse);
+            });
+        }
+        __syncthreads();
+    }
+}
+
+// the splits of a row together, one wave a row: a lane has a split, and the largest of the splits' heads is the next of the top
+__global__ void __launch_bounds__(64) log_prob_join_kernel(const LogProbArgs p) {
+    __shared__ uint64_t heads[64 * kMostTop];
+    const uint32_t lane = threadIdx.x;
+    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const bool in = lane < p.splits;
+        const float *part = p.partial + ((size_t)row * p.splits + (in ? lane : 0)) * log_prob_part(p.top);
+        Sums sums{in ? part[0] : kMinusInf, in ? part[1] : 0.0f, in ? part[2] : 0.0f};
+        const float m = wave_max(sums.m);
+        sums.raise(m);
+        const float s = lanes_sum<64>(sums.s), t = lanes_sum<64>(sums.t), lse = s == 0.0f ? kMinusInf : m + logf(s);
+        if (lane == 0) log_prob_finish(p, row, m, s, t);
+        if (!p.top) continue;
+        for (uint32_t i = lane; i < p.splits * p.top; i += 64)
+            heads[i] = ((const uint64_t *)(p.partial + ((size_t)row * p.splits + i / p.top) * log_prob_part(p.top) + 4))[i % p.top];
+        __syncthreads();
+        const uint64_t *own = heads + lane * p.top;
+        uint32_t next = 0;
+        uint64_t head = in ? own[0] : 0;
+        for (uint32_t i = 0; i < p.top; ++i) {
+            uint64_t most = head;
+            most = larger(most, key_dpp<0xB1>(most));
+            most = larger(most, key_dpp<0x4E>(most));
+            most = larger(most, key_dpp<0x141>(most));
+            most = larger(most, key_dpp<0x140>(most));
+            most = larger(larger(key_lane(most, 0), key_lane(most, 16)), larger(key_lane(most, 32), key_lane(most, 48)));
+            if (head == most && head != 0) {
+                store_top(p, row, i, most, lse);
+                ++next;
+                head = next < p.top ? own[next] : 0;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- backward: a workgroup takes kLogProbTurn columns a turn
+template <int DT>
+__global__ void __launch_bounds__(kLogProbThreads) log_prob_backward_kernel(const LogProbBackwardArgs p) {
+    for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
+        const char *x = (const char *)p.logits + (size_t)row * p.ld * Octet<DT>::ES;
+        char *dx = (char *)p.dlogits + (size_t)row * p.ldd * dtype_bytes(p.out_dt);
+        const int64_t token = token_at(p.tokens, p.token_bytes, row);
+        const bool asked = token >= 0 && token < (int64_t)p.cols;
+        const float lse = p.lse[row], b = p.dentropy ? p.dentropy[row] : 0.0f, h = b != 0.0f ? p.entropy[row] : 0.0f;
+        const bool none = lse == kMinusInf;
+        const float a = asked && !none ? p.dlogp[row] : 0.0f;
+        for (uint32_t c = (blockIdx.x * kLogProbThreads + threadIdx.x) * kOctet; c < p.cols; c += gridDim.x * kLogProbTurn) {
+            Octet<DT> o;
+            float v[8];
+            o.request(x, c, p.cols);
+            o.settle(c, p.cols);
+            o.floats(v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float l = v[e] - lse, q = none ? 0.0f : exp_of(l);
+                const float g = a + b * (__builtin_fmaxf(l, kNothing) + h);
+                v[e] = -(q * g);
+                if (asked && (int64_t)(c + e) == token) v[e] += a;
+            }
+            if (none)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+            store_octet(dx, p.out_dt, c, p.cols, v);
+        }
+    }
+}
+
+}  // namespace qgemm

@@ -8,25 +8,6 @@
 
 namespace qgemm {
 
-// sums of N values over a workgroup of WAVES waves, in every lane; `red` is free again after the next barrier behind this
-template <int WAVES, int N>
-__device__ __forceinline__ void workgroup_sums(float (&v)[N], float (*red)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = lanes_sum<64>(v[i]);
-    if constexpr (WAVES > 1) {
-        if ((threadIdx.x & 63) == 0)
-#pragma unroll
-            for (int i = 0; i < N; ++i) red[threadIdx.x >> 6][i] = v[i];
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            v[i] = red[0][i];
-#pragma unroll
-            for (int w = 1; w < WAVES; ++w) v[i] += red[w][i];
-        }
-    }
-}
-
 // x - mean for the elements that the row has, zeros behind it
 __device__ __forceinline__ void centre(float (&v)[8], float mean, uint32_t c, uint32_t cols) {
 #pragma unroll

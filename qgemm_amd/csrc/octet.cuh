@@ -197,6 +197,24 @@ __device__ __forceinline__ float lanes_sum(float v) {
     }
     return v;
 }
+// sums of N values over a workgroup of WAVES waves, in every lane; `red` is free again after the next barrier behind this
+template <int WAVES, int N>
+__device__ __forceinline__ void workgroup_sums(float (&v)[N], float (*red)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = lanes_sum<64>(v[i]);
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) red[threadIdx.x >> 6][i] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = red[0][i];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) v[i] += red[w][i];
+        }
+    }
+}
 // largest |v| of the 128 columns that 16 neighbouring lanes hold, as bits: their order is that of the numbers, with infinity and NaNs on top
 __device__ __forceinline__ uint32_t block_max_bits(const float (&v)[8]) {
     uint32_t m = 0;

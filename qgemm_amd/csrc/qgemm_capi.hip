@@ -17,6 +17,7 @@
 #include "quant_kernels.cuh"
 #include "selftest.cuh"
 #include "training.h"
+#include "model.h"
 #include "variants.h"
 
 using namespace qgemm;
@@ -1824,6 +1825,53 @@ int keep_entry(bool encode, int in_dt, int out_dt, const void *in, size_t ld_in,
     return e == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
 }
 
+// ---- adapters
+int adapters_size_status(size_t rows, size_t adapters, size_t rank, size_t k, size_t n) {
+    if (adapters == 0 || rank == 0 || k == 0 || n == 0) return QGEMM_ERR_INVALID_ARG;
+    if (rows >= ((size_t)1 << 28) || adapters > kMostAdapters || rank > kMostRank) return QGEMM_ERR_TOO_LARGE;
+    if (k > (size_t)kMaxGridY * 256 || n > (size_t)kMaxGridY * 256) return QGEMM_ERR_TOO_LARGE;       // (columns are the y extent of launches)
+    return QGEMM_OK;
+}
+ShrinkArgs shrink_args(int dtype, const void *groups, const void *x, size_t ldx, const void *w, size_t rows, size_t adapters, size_t rank, size_t cols) {
+    ShrinkArgs s;
+    std::memset(&s, 0, sizeof(s));
+    s.g = row_groups(groups, rows, adapters);
+    s.x = x, s.w = w;
+    s.ldx = ldx;
+    s.cols = (uint32_t)cols, s.rank = (uint32_t)rank;
+    s.dt = dtype;
+    return s;
+}
+// Where the sums over the rank go: `u`, [rows][rank], where the caller wants them and they come in one part, else into the workspace, of
+// which the bytes are returned
+size_t plan_rank_sums(ShrinkArgs &s, float *u) {
+    s.u.planes = plan_shrink(s, g_ctx.num_cus);
+    s.part = (uint32_t)(((s.cols + s.u.planes - 1) / s.u.planes + 255) / 256 * 256);
+    s.u.planes = (s.cols + s.part - 1) / s.part;
+    if (u && s.u.planes == 1) {
+        s.u.at = u;
+        s.u.pitch = s.rank;
+        s.zero = 1;
+        return 0;
+    }
+    s.u.pitch = rank_pitch(s.rank);
+    s.u.stride = (uint64_t)s.g.rows * s.u.pitch;
+    return s.u.planes * s.u.stride * sizeof(float);
+}
+ExpandArgs expand_args(const ShrinkArgs &s, int y_dtype, const void *w, const float *scaling, const void *y, size_t ldy, void *out, size_t ldo, size_t cols) {
+    ExpandArgs e;
+    std::memset(&e, 0, sizeof(e));
+    e.g = s.g;
+    e.w = w, e.y = y;
+    e.scaling = scaling;
+    e.out = out;
+    e.u = s.u;
+    e.ldy = ldy, e.ldo = ldo;
+    e.cols = (uint32_t)cols, e.rank = s.rank;
+    e.dt = s.dt, e.y_dt = y_dtype;
+    return e;
+}
+
 }  // namespace
 
 // ===========================================================================
@@ -2194,6 +2242,212 @@ QGEMM_EXPORT int qgemm_weight_gradient(int dy_dtype, int q_dtype, int dw_dtype, 
     g_ctx.last_config = a.tile == TILE_256x256 ? "weight_gradient_256x256" : a.tile == TILE_256x128 ? "weight_gradient_256x128" : "weight_gradient_128x128";
     if (a.slices > 1) g_ctx.last_config += "_split" + std::to_string(a.slices);
     return launch_weight_grad(a, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+}
+
+// ---- root-mean-square norm, adapters beside a product, log probabilities
+QGEMM_EXPORT int qgemm_rms_norm(int x_dtype, int residual_dtype, int y_dtype, int param_dtype, int q_dtype, const void *x, size_t ldx, const void *residual,
+                                size_t ldr, const void *weight, float eps, void *h, size_t ldh, void *y, size_t ldy, float *rstd, void *q, size_t ldq,
+                                float *scales, size_t rows, size_t cols, void *stream) {
+    if (!is_float_type(x_dtype) || (residual && !is_float_type(residual_dtype)) || (y && !is_float_type(y_dtype))) return QGEMM_ERR_UNSUPPORTED;
+    if ((weight && !is_float_type(param_dtype)) || (q && !is_code_type(q_dtype))) return QGEMM_ERR_UNSUPPORTED;
+    if (cols == 0 || !(eps >= 0.0f) || (!residual) != (!h) || (!q) != (!scales)) return QGEMM_ERR_INVALID_ARG;
+    if (rows >= ((size_t)1 << 31) || cols >= ((size_t)1 << 31)) return QGEMM_ERR_TOO_LARGE;
+    if (rows == 0) return QGEMM_OK;
+    if (!x || (!y && !q) || ldx < cols || (residual && (ldr < cols || ldh < cols)) || (y && ldy < cols) || (q && ldq < cols)) return QGEMM_ERR_INVALID_ARG;
+    std::lock_guard<std::mutex> lock(g_ctx.mu);
+    const int st = ensure_init_locked();
+    if (st != QGEMM_OK) return st;
+    RmsArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.x = x, a.residual = residual, a.weight = weight;
+    a.h = h, a.y = y, a.q = q;
+    a.rstd = rstd, a.scales = scales;
+    a.ldx = ldx, a.ldr = ldr, a.ldh = ldh, a.ldy = ldy, a.ldq = ldq;
+    a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.kb = blocks_of(cols);
+    a.eps = eps;
+    a.x_dt = x_dtype, a.r_dt = residual ? residual_dtype : x_dtype, a.y_dt = y_dtype, a.param_dt = param_dtype, a.q_dt = q_dtype;
+    g_ctx.last_config = "rms_norm";
+    return launch_rms_norm(a, g_ctx.num_cus, (hipStream_t)stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+}
+
+QGEMM_EXPORT int qgemm_rms_norm_backward(int dy_dtype, int h_dtype, int dh_dtype, int dx_dtype, int param_dtype, const void *dy, size_t lddy, const void *h,
+                                         size_t ldh, const float *rstd, const void *weight, const void *dh, size_t lddh, void *dx, size_t lddx,
+                                         void *dweight, size_t rows, size_t cols, void *stream_) {
+    if (!is_float_type(dy_dtype) || !is_float_type(h_dtype) || !is_float_type(dx_dtype) || (dh && !is_float_type(dh_dtype))) return QGEMM_ERR_UNSUPPORTED;
+    if ((weight || dweight) && !is_float_type(param_dtype)) return QGEMM_ERR_UNSUPPORTED;
+    if (cols == 0) return QGEMM_ERR_INVALID_ARG;
+    if (rows >= ((size_t)1 << 31) || cols >= ((size_t)1 << 31)) return QGEMM_ERR_TOO_LARGE;
+    if (dweight && cols > ((size_t)1 << 31) - 128) return QGEMM_ERR_TOO_LARGE;      // (2^32 threads of the columns' sums)
+    if (rows && (!dy || !h || !dx || !rstd || lddy < cols || ldh < cols || lddx < cols || (dh && lddh < cols))) return QGEMM_ERR_INVALID_ARG;
+    if (rows == 0 && !dweight) return QGEMM_OK;
+    hipStream_t stream = (hipStream_t)stream_;
+    std::lock_guard<std::mutex> lock(g_ctx.mu);
+    int st = ensure_init_locked();
+    if (st != QGEMM_OK) return st;
+    WorkspaceUse ws_use(stream);
+    RmsBackwardArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.dy = dy, a.h = h, a.dh = dh, a.weight = weight;
+    a.rstd = rstd;
+    a.dx = dx, a.dweight = dweight;
+    a.lddy = lddy, a.ldh = ldh, a.lddh = lddh, a.lddx = lddx;
+    a.rows = (uint32_t)rows, a.cols = (uint32_t)cols;
+    a.dy_dt = dy_dtype, a.h_dt = h_dtype, a.dh_dt = dh_dtype, a.dx_dt = dx_dtype, a.param_dt = param_dtype;
+    a.groups = rms_backward_groups(a, g_ctx.num_cus);
+    if (a.groups) {
+        void *ws = nullptr;
+        st = ensure_workspace_locked(rms_partial_bytes(a.groups, a.cols), stream, &ws);
+        if (st != QGEMM_OK) return st;
+        a.partial = (float *)ws;
+    }
+    g_ctx.last_config = "rms_norm_backward";
+    return launch_rms_norm_backward(a, g_ctx.num_cus, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+}
+
+QGEMM_EXPORT int qgemm_group_rows_words(size_t rows, size_t adapters, size_t *words) {
+    if (!words || adapters == 0) return QGEMM_ERR_INVALID_ARG;
+    if (rows >= ((size_t)1 << 28) || adapters > kMostAdapters) return QGEMM_ERR_TOO_LARGE;
+    *words = group_words(rows, adapters);
+    return QGEMM_OK;
+}
+
+QGEMM_EXPORT int qgemm_group_rows(int id_bytes, const void *ids, size_t rows, size_t adapters, void *groups, void *stream) {
+    if (id_bytes != 4 && id_bytes != 8) return QGEMM_ERR_UNSUPPORTED;
+    if (adapters == 0) return QGEMM_ERR_INVALID_ARG;
+    if (rows >= ((size_t)1 << 28) || adapters > kMostAdapters) return QGEMM_ERR_TOO_LARGE;
+    if (!groups || (uintptr_t)groups % 8 || (rows && !ids)) return QGEMM_ERR_INVALID_ARG;
+    std::lock_guard<std::mutex> lock(g_ctx.mu);
+    const int st = ensure_init_locked();
+    if (st != QGEMM_OK) return st;
+    g_ctx.last_config = "group_rows";
+    return launch_group_rows(ids, id_bytes, row_groups(groups, rows, adapters), (hipStream_t)stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+}
+
+QGEMM_EXPORT int qgemm_add_adapters(int dtype, int y_dtype, const void *y, size_t ldy, const void *x, size_t ldx, const void *A, const void *B,
+                                    const float *scaling, const void *groups, void *out, size_t ldo, float *u, size_t rows, size_t adapters,
+                                    size_t rank, size_t k, size_t n, void *stream_) {
+    if ((dtype != QGEMM_DT_BF16 && dtype != QGEMM_DT_F16) || !is_float_type(y_dtype)) return QGEMM_ERR_UNSUPPORTED;
+    int st = adapters_size_status(rows, adapters, rank, k, n);
+    if (st != QGEMM_OK) return st;
+    if (rows == 0) return QGEMM_OK;
+    if (!y || !x || !A || !B || !groups || (uintptr_t)groups % 8 || !out || ldy < n || ldx < k || ldo < n || (out == y && ldo != ldy)) return QGEMM_ERR_INVALID_ARG;
+    hipStream_t stream = (hipStream_t)stream_;
+    std::lock_guard<std::mutex> lock(g_ctx.mu);
+    st = ensure_init_locked();
+    if (st != QGEMM_OK) return st;
+    WorkspaceUse ws_use(stream);
+    ShrinkArgs s = shrink_args(dtype, groups, x, ldx, A, rows, adapters, rank, k);
+    const size_t room = plan_rank_sums(s, u);
+    if (room) {
+        void *ws = nullptr;
+        st = ensure_workspace_locked(room, stream, &ws);
+        if (st != QGEMM_OK) return st;
+        s.u.at = (float *)ws;
+    }
+    ExpandArgs e = expand_args(s, y_dtype, B, scaling, y, ldy, out, ldo, n);
+    e.keep = room ? u : nullptr;
+    g_ctx.last_config = "add_adapters";
+    if (launch_shrink(s, stream) != hipSuccess) return QGEMM_ERR_LAUNCH;
+    return launch_expand(e, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+}
+
+QGEMM_EXPORT int qgemm_add_adapters_backward(int dtype, int dx_dtype, int grad_dtype, const void *dy, size_t lddy, const void *x, size_t ldx, const float *u,
+                                             const void *A, const void *B, const float *scaling, const void *groups, const void *dx0, size_t lddx0,
+                                             void *dx, size_t lddx, void *dA, void *dB, size_t rows, size_t adapters, size_t rank, size_t k, size_t n,
+                                             void *stream_) {
+    if ((dtype != QGEMM_DT_BF16 && dtype != QGEMM_DT_F16) || !is_float_type(grad_dtype) || (dx && !is_float_type(dx_dtype))) return QGEMM_ERR_UNSUPPORTED;
+    int st = adapters_size_status(rows, adapters, rank, k, n);
+    if (st != QGEMM_OK) return st;
+    if (rows == 0 && !dA && !dB) return QGEMM_OK;
+    if (!groups || (uintptr_t)groups % 8) return QGEMM_ERR_INVALID_ARG;
+    if (rows && (!dy || !x || !A || !B || lddy < n || ldx < k || (dB && !u) || (dx0 && !dx) || (dx && lddx < k) || (dx0 && lddx0 < k) ||
+                 (dx0 && dx0 == dx && lddx0 != lddx)))
+        return QGEMM_ERR_INVALID_ARG;
+    hipStream_t stream = (hipStream_t)stream_;
+    std::lock_guard<std::mutex> lock(g_ctx.mu);
+    st = ensure_init_locked();
+    if (st != QGEMM_OK) return st;
+    WorkspaceUse ws_use(stream);
+    ShrinkArgs s = shrink_args(dtype, groups, dy, lddy, B, rows, adapters, rank, n);
+    const size_t sums = rows && (dx || dA) ? (plan_rank_sums(s, nullptr) + 255) / 256 * 256 : 0;
+    auto gradient = [&](const void *z, size_t ldz, size_t cols, RankSums of, void *dw) {
+        AdapterGradArgs g;
+        std::memset(&g, 0, sizeof(g));
+        g.g = s.g;
+        g.z = z, g.scaling = scaling, g.dw = dw;
+        g.u = of;
+        g.ldz = ldz;
+        g.cols = (uint32_t)cols, g.rank = (uint32_t)rank;
+        g.dt = dtype, g.dw_dt = grad_dtype;
+        return g;
+    };
+    AdapterGradArgs ga = gradient(x, ldx, k, s.u, dA), gb = gradient(dy, lddy, n, RankSums{const_cast<float *>(u), 0, (uint32_t)rank, 1}, dB);
+    const size_t room = std::max(dA ? plan_adapter_grad(ga, g_ctx.num_cus) : 0, dB ? plan_adapter_grad(gb, g_ctx.num_cus) : 0);
+    if (sums + room) {
+        void *ws = nullptr;
+        st = ensure_workspace_locked(sums + room, stream, &ws);
+        if (st != QGEMM_OK) return st;
+        s.u.at = ga.u.at = (float *)ws;
+        ga.room = gb.room = (float *)((char *)ws + sums);
+    }
+    g_ctx.last_config = "add_adapters_backward";
+    if (sums && launch_shrink(s, stream) != hipSuccess) return QGEMM_ERR_LAUNCH;
+    if (rows && dx && launch_expand(expand_args(s, dx_dtype, A, scaling, dx0, dx0 ? lddx0 : lddx, dx, lddx, k), stream) != hipSuccess) return QGEMM_ERR_LAUNCH;
+    if (dA && launch_adapter_grad(ga, stream) != hipSuccess) return QGEMM_ERR_LAUNCH;
+    return !dB || launch_adapter_grad(gb, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+}
+
+QGEMM_EXPORT int qgemm_log_probabilities(int dtype, int token_bytes, const void *logits, size_t ld, const void *tokens, int top, float *logp, float *entropy,
+                                         float *lse, float *values, int64_t *indices, size_t rows, size_t cols, void *stream_) {
+    if (!is_float_type(dtype) || (token_bytes != 4 && token_bytes != 8)) return QGEMM_ERR_UNSUPPORTED;
+    if (cols == 0 || top < 0 || (size_t)top > cols) return QGEMM_ERR_INVALID_ARG;
+    if (rows >= ((size_t)1 << 31) || cols >= ((size_t)1 << 31) || top > (int)kMostTop) return QGEMM_ERR_TOO_LARGE;
+    if (rows == 0) return QGEMM_OK;
+    if (!logits || !tokens || !logp || !entropy || !lse || (top && (!values || !indices)) || ld < cols) return QGEMM_ERR_INVALID_ARG;
+    hipStream_t stream = (hipStream_t)stream_;
+    std::lock_guard<std::mutex> lock(g_ctx.mu);
+    int st = ensure_init_locked();
+    if (st != QGEMM_OK) return st;
+    WorkspaceUse ws_use(stream);
+    LogProbArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.logits = logits, a.tokens = tokens;
+    a.logp = logp, a.entropy = entropy, a.lse = lse, a.values = values;
+    a.indices = indices;
+    a.ld = ld;
+    a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.top = (uint32_t)top;
+    a.dt = dtype, a.token_bytes = token_bytes;
+    if (const size_t room = plan_log_prob(a, g_ctx.num_cus)) {
+        void *ws = nullptr;
+        st = ensure_workspace_locked(room, stream, &ws);
+        if (st != QGEMM_OK) return st;
+        a.partial = (float *)ws;
+    }
+    g_ctx.last_config = "log_probabilities";
+    return launch_log_prob(a, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+}
+
+QGEMM_EXPORT int qgemm_log_probabilities_backward(int dtype, int out_dtype, int token_bytes, const void *logits, size_t ld, const void *tokens, const float *lse,
+                                                  const float *entropy, const float *dlogp, const float *dentropy, void *dlogits, size_t ldd, size_t rows,
+                                                  size_t cols, void *stream) {
+    if (!is_float_type(dtype) || !is_float_type(out_dtype) || (token_bytes != 4 && token_bytes != 8)) return QGEMM_ERR_UNSUPPORTED;
+    if (cols == 0) return QGEMM_ERR_INVALID_ARG;
+    if (rows >= ((size_t)1 << 31) || cols >= ((size_t)1 << 31)) return QGEMM_ERR_TOO_LARGE;
+    if (rows == 0) return QGEMM_OK;
+    if (!logits || !tokens || !lse || !dlogp || (dentropy && !entropy) || !dlogits || ld < cols || ldd < cols) return QGEMM_ERR_INVALID_ARG;
+    std::lock_guard<std::mutex> lock(g_ctx.mu);
+    const int st = ensure_init_locked();
+    if (st != QGEMM_OK) return st;
+    LogProbBackwardArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.logits = logits, a.tokens = tokens;
+    a.lse = lse, a.entropy = entropy, a.dlogp = dlogp, a.dentropy = dentropy;
+    a.dlogits = dlogits;
+    a.ld = ld, a.ldd = ldd;
+    a.rows = (uint32_t)rows, a.cols = (uint32_t)cols;
+    a.dt = dtype, a.out_dt = out_dtype, a.token_bytes = token_bytes;
+    g_ctx.last_config = "log_probabilities_backward";
+    return launch_log_prob_backward(a, (hipStream_t)stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
 }
 
 QGEMM_EXPORT int qgemm_gemm(int in_dtype, int out_dtype, int layout_b, const void *A, size_t ldA, const void *B, size_t ldB,

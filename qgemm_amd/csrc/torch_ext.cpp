@@ -4,6 +4,7 @@
 // every function checks its tensors and forwards their data pointers, with torch's current stream, to the
 // C ABI of libqgemm.so.
 #include <torch/extension.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
@@ -330,6 +331,177 @@ std::tuple<int, at::Tensor, at::Tensor> ops_weight_gradient(const at::Tensor &dy
             dw, db};
 }
 
+// ---- beside the products of a language model: all tensors on the current device
+bool here(const at::Tensor &t) { return t.is_cuda() && t.get_device() == c10::hip::current_device(); }
+bool here(const std::optional<at::Tensor> &t) { return !t || here(*t); }
+bool rows_like(const at::Tensor &t, int64_t rows, int64_t cols, int64_t &ld) {
+    int64_t r, c;
+    return here(t) && rows_of(t, r, c, ld) && r == rows && c == cols;
+}
+int token_bytes(const at::Tensor &t) { return t.scalar_type() == at::kLong ? 8 : t.scalar_type() == at::kInt ? 4 : 0; }
+void *data_or_null(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// (status, y, h, rstd, q, scales)
+typedef std::tuple<int, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> RmsOut;
+RmsOut ops_rms_norm(const at::Tensor &x, const std::optional<at::Tensor> &weight, double eps, const std::optional<at::Tensor> &residual,
+                    std::optional<at::ScalarType> out, std::optional<at::ScalarType> codes, bool store_y) {
+    RmsOut r;
+    std::get<0>(r) = kNotPlain;
+    int64_t rows, cols, ld, ldr = 0;
+    int pdt;
+    if (!here(x) || !here(weight) || !rows_of(x, rows, cols, ld) || !parameters_ok(weight, std::nullopt, cols, pdt)) return r;
+    const int xdt = plain_dtype(x, false), qdt = codes ? code_dtype(*codes) : 0;
+    if (!float_dtype(xdt) || qdt < 0 || (!store_y && !codes)) return r;
+    int rdt = xdt, ydt = xdt;
+    at::Tensor h = x, y, q, scales;
+    if (residual) {
+        rdt = plain_dtype(*residual, false);
+        if (!float_dtype(rdt) || !rows_like(*residual, rows, cols, ldr)) return r;
+        h = at::empty(x.sizes(), residual->options());
+    }
+    if (out && *out != at::kFloat && *out != at::kBFloat16 && *out != at::kHalf) return r;
+    if (store_y) {
+        y = at::empty(x.sizes(), out ? x.options().dtype(*out) : x.options());
+        ydt = plain_dtype(y, false);
+    }
+    const auto f32 = x.options().dtype(at::kFloat);
+    at::Tensor rstd = at::empty(x.sizes().slice(0, x.dim() - 1), f32);
+    if (codes) {
+        q = at::empty(x.sizes(), x.options().dtype(*codes));
+        scales = at::empty(with_last(x, (cols + 127) / 128), f32);
+    }
+    int st;
+    {
+        py::gil_scoped_release no_gil;
+        st = qgemm_rms_norm(xdt, rdt, ydt, pdt, qdt, x.data_ptr(), ld, data_or_null(residual), ldr, data_or_null(weight), (float)eps,
+                            residual ? h.data_ptr() : nullptr, cols, data_or_null(y), cols, (float *)rstd.data_ptr(), data_or_null(q), cols,
+                            (float *)data_or_null(scales), rows, cols, current_stream());
+    }
+    return {st, y, h, rstd, q, scales};
+}
+
+// (status, dx, dweight)
+std::tuple<int, at::Tensor, at::Tensor> ops_rms_norm_backward(const at::Tensor &dy, const at::Tensor &h, const at::Tensor &rstd, const std::optional<at::Tensor> &weight,
+                                                              const std::optional<at::Tensor> &dh, std::optional<at::ScalarType> out) {
+    const std::tuple<int, at::Tensor, at::Tensor> not_plain{kNotPlain, at::Tensor(), at::Tensor()};
+    int64_t rows, cols, lddy, ldh, lddh = 0;
+    int pdt;
+    if (!here(dy) || !here(rstd) || !here(weight) || !rows_of(dy, rows, cols, lddy) || !rows_like(h, rows, cols, ldh) || (dh && !rows_like(*dh, rows, cols, lddh)) ||
+        !parameters_ok(weight, std::nullopt, cols, pdt) || !float_vector(rstd, rows))
+        return not_plain;
+    const int dydt = plain_dtype(dy, false), hdt = plain_dtype(h, false), dhdt = dh ? plain_dtype(*dh, false) : QGEMM_DT_F32;
+    if (!float_dtype(dydt) || !float_dtype(hdt) || !float_dtype(dhdt) || (out && *out != at::kFloat && *out != at::kBFloat16 && *out != at::kHalf)) return not_plain;
+    at::Tensor dx = at::empty(dy.sizes(), out ? dy.options().dtype(*out) : dy.options()), dw;
+    if (weight) dw = at::empty_like(*weight);
+    py::gil_scoped_release no_gil;
+    return {qgemm_rms_norm_backward(dydt, hdt, dhdt, plain_dtype(dx, false), pdt, dy.data_ptr(), lddy, h.data_ptr(), ldh, (const float *)rstd.data_ptr(),
+                                    data_or_null(weight), data_or_null(dh), lddh, dx.data_ptr(), cols, data_or_null(dw), rows, cols, current_stream()),
+            dx, dw};
+}
+
+// (status, words)
+std::tuple<int, at::Tensor> ops_group_rows(const at::Tensor &ids, int64_t adapters) {
+    const int bytes = token_bytes(ids);
+    size_t words;
+    if (!here(ids) || !bytes || !ids.is_contiguous() || adapters < 1 || qgemm_group_rows_words(ids.numel(), adapters, &words) != QGEMM_OK)
+        return {kNotPlain, at::Tensor()};
+    at::Tensor out = at::empty({(int64_t)words}, ids.options().dtype(at::kInt));
+    py::gil_scoped_release no_gil;
+    return {qgemm_group_rows(bytes, ids.data_ptr(), ids.numel(), adapters, out.data_ptr(), current_stream()), out};
+}
+
+// a factor of the adapters, [adapters][rank][cols]
+bool factor_ok(const at::Tensor &w, const at::Tensor &x, int64_t adapters, int64_t &rank, int64_t &cols) {
+    if (!here(w) || w.scalar_type() != x.scalar_type() || w.dim() != 3 || !w.is_contiguous() || w.size(0) != adapters) return false;
+    rank = w.size(1);
+    cols = w.size(2);
+    return adapters > 0 && rank > 0 && cols > 0;
+}
+
+// (status, out, u)
+std::tuple<int, at::Tensor, at::Tensor> ops_add_adapters(const at::Tensor &y, const at::Tensor &x, const at::Tensor &A, const at::Tensor &B, const at::Tensor &words,
+                                                         int64_t rows, int64_t adapters, const std::optional<at::Tensor> &scaling,
+                                                         const std::optional<at::Tensor> &into, bool keep) {
+    const std::tuple<int, at::Tensor, at::Tensor> not_plain{kNotPlain, at::Tensor(), at::Tensor()};
+    int64_t xrows, k, ldx, rank, rank_b, ka, n, ldy, ldo;
+    const int dt = plain_dtype(x, false), ydt = plain_dtype(y, false);
+    if ((dt != QGEMM_DT_BF16 && dt != QGEMM_DT_F16) || !float_dtype(ydt) || !here(x) || !here(words) || !here(scaling) || !rows_of(x, xrows, k, ldx) || xrows != rows ||
+        !factor_ok(A, x, adapters, rank, ka) || !factor_ok(B, x, adapters, rank_b, n) || ka != k || rank_b != rank || !rows_like(y, rows, n, ldy) ||
+        (scaling && !float_vector(*scaling, adapters)))
+        return not_plain;
+    at::Tensor out = into ? *into : at::empty(y.sizes(), y.options()), u;
+    if (out.scalar_type() != y.scalar_type() || out.sizes() != y.sizes() || !rows_like(out, rows, n, ldo)) return not_plain;
+    if (keep) u = at::empty(with_last(x, rank), x.options().dtype(at::kFloat));
+    py::gil_scoped_release no_gil;
+    return {qgemm_add_adapters(dt, ydt, y.data_ptr(), ldy, x.data_ptr(), ldx, A.data_ptr(), B.data_ptr(), (const float *)data_or_null(scaling), words.data_ptr(),
+                               out.data_ptr(), ldo, (float *)data_or_null(u), rows, adapters, rank, k, n, current_stream()),
+            out, u};
+}
+
+// (status, dx, dA, dB)
+std::tuple<int, at::Tensor, at::Tensor, at::Tensor> ops_add_adapters_backward(const at::Tensor &dy, const at::Tensor &x, const at::Tensor &u, const at::Tensor &A,
+                                                                              const at::Tensor &B, const at::Tensor &words, int64_t rows, int64_t adapters,
+                                                                              const std::optional<at::Tensor> &scaling, const std::optional<at::Tensor> &dx0,
+                                                                              at::ScalarType grad) {
+    const std::tuple<int, at::Tensor, at::Tensor, at::Tensor> not_plain{kNotPlain, at::Tensor(), at::Tensor(), at::Tensor()};
+    int64_t xrows, k, ldx, rank, rank_b, ka, n, lddy, ld0 = 0;
+    const int dt = plain_dtype(x, false), dxdt = dx0 ? plain_dtype(*dx0, false) : dt;
+    if ((dt != QGEMM_DT_BF16 && dt != QGEMM_DT_F16) || !float_dtype(dxdt) || !here(x) || !here(u) || !here(words) || !here(scaling) || !rows_of(x, xrows, k, ldx) ||
+        xrows != rows || !factor_ok(A, x, adapters, rank, ka) || !factor_ok(B, x, adapters, rank_b, n) || ka != k || rank_b != rank ||
+        dy.scalar_type() != x.scalar_type() || !rows_like(dy, rows, n, lddy) || !float_vector(u, rows * rank) || (dx0 && !rows_like(*dx0, rows, k, ld0)) ||
+        (scaling && !float_vector(*scaling, adapters)) || (grad != at::kFloat && grad != at::kBFloat16 && grad != at::kHalf))
+        return not_plain;
+    at::Tensor dx = at::empty(x.sizes(), dx0 ? dx0->options() : x.options()), dA = at::empty(A.sizes(), A.options().dtype(grad)), dB = at::empty(B.sizes(), B.options().dtype(grad));
+    py::gil_scoped_release no_gil;
+    return {qgemm_add_adapters_backward(dt, dxdt, plain_dtype(dA, false), dy.data_ptr(), lddy, x.data_ptr(), ldx, (const float *)u.data_ptr(), A.data_ptr(), B.data_ptr(),
+                                        (const float *)data_or_null(scaling), words.data_ptr(), data_or_null(dx0), ld0, dx.data_ptr(), k, dA.data_ptr(), dB.data_ptr(), rows,
+                                        adapters, rank, k, n, current_stream()),
+            dx, dA, dB};
+}
+
+// (status, logp, entropy, lse, values, indices)
+RmsOut ops_log_probabilities(const at::Tensor &logits, const at::Tensor &tokens, int64_t top) {
+    RmsOut r;
+    std::get<0>(r) = kNotPlain;
+    int64_t rows, cols, ld;
+    const int dt = plain_dtype(logits, false), bytes = token_bytes(tokens);
+    if (!here(logits) || !here(tokens) || !float_dtype(dt) || !bytes || !rows_of(logits, rows, cols, ld) || tokens.numel() != rows || !tokens.is_contiguous() || top < 0 ||
+        top > 32)
+        return r;
+    const auto f32 = logits.options().dtype(at::kFloat);
+    const at::IntArrayRef lead = logits.sizes().slice(0, logits.dim() - 1);
+    at::Tensor logp = at::empty(lead, f32), entropy = at::empty(lead, f32), lse = at::empty(lead, f32), values, indices;
+    if (top) {
+        values = at::empty(with_last(logits, top), f32);
+        indices = at::empty(with_last(logits, top), logits.options().dtype(at::kLong));
+    }
+    int st;
+    {
+        py::gil_scoped_release no_gil;
+        st = qgemm_log_probabilities(dt, bytes, logits.data_ptr(), ld, tokens.data_ptr(), (int)top, (float *)logp.data_ptr(), (float *)entropy.data_ptr(),
+                                     (float *)lse.data_ptr(), (float *)data_or_null(values), (int64_t *)data_or_null(indices), rows, cols, current_stream());
+    }
+    return {st, logp, entropy, lse, values, indices};
+}
+
+// (status, dlogits)
+std::tuple<int, at::Tensor> ops_log_probabilities_backward(const at::Tensor &logits, const at::Tensor &tokens, const at::Tensor &lse, const std::optional<at::Tensor> &entropy,
+                                                           const at::Tensor &dlogp, const std::optional<at::Tensor> &dentropy, std::optional<at::ScalarType> out) {
+    int64_t rows, cols, ld;
+    const int dt = plain_dtype(logits, false), bytes = token_bytes(tokens);
+    auto vector = [&](const at::Tensor &t) { return here(t) && float_vector(t, rows); };
+    if (!here(logits) || !here(tokens) || !float_dtype(dt) || !bytes || !rows_of(logits, rows, cols, ld) || tokens.numel() != rows || !tokens.is_contiguous() ||
+        !vector(lse) || !vector(dlogp) || (entropy && !vector(*entropy)) || (dentropy && !vector(*dentropy)) ||
+        (out && *out != at::kFloat && *out != at::kBFloat16 && *out != at::kHalf))
+        return {kNotPlain, at::Tensor()};
+    at::Tensor dx = at::empty(logits.sizes(), out ? logits.options().dtype(*out) : logits.options());
+    py::gil_scoped_release no_gil;
+    return {qgemm_log_probabilities_backward(dt, plain_dtype(dx, false), bytes, logits.data_ptr(), ld, tokens.data_ptr(), (const float *)lse.data_ptr(),
+                                             (const float *)data_or_null(entropy), (const float *)dlogp.data_ptr(), (const float *)data_or_null(dentropy), dx.data_ptr(),
+                                             cols, rows, cols, current_stream()),
+            dx};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -347,4 +519,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("ops_checkpoint", &ops_checkpoint);
     m.def("ops_restore", &ops_restore);
     m.def("ops_weight_gradient", &ops_weight_gradient);
+    m.def("ops_rms_norm", &ops_rms_norm);
+    m.def("ops_rms_norm_backward", &ops_rms_norm_backward);
+    m.def("ops_group_rows", &ops_group_rows);
+    m.def("ops_add_adapters", &ops_add_adapters);
+    m.def("ops_add_adapters_backward", &ops_add_adapters_backward);
+    m.def("ops_log_probabilities", &ops_log_probabilities);
+    m.def("ops_log_probabilities_backward", &ops_log_probabilities_backward);
 }

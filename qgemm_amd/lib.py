@@ -49,6 +49,15 @@ SIGNATURES = {
     "qgemm_checkpoint": (_i, [_i, _i, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _vp]),
     "qgemm_restore": (_i, [_i, _i, _vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp]),
     "qgemm_weight_gradient": (_i, [_i, _i, _i, _i, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz, _vp]),
+    "qgemm_rms_norm": (_i, [_i, _i, _i, _i, _i, _vp, _sz, _vp, _sz, _vp, C.c_float, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _sz, _sz, _vp]),
+    "qgemm_rms_norm_backward": (_i, [_i, _i, _i, _i, _i, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _vp]),
+    "qgemm_group_rows_words": (_i, [_sz, _sz, C.POINTER(_sz)]),
+    "qgemm_group_rows": (_i, [_i, _vp, _sz, _sz, _vp, _vp]),
+    "qgemm_add_adapters": (_i, [_i, _i, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _sz, _vp]),
+    "qgemm_add_adapters_backward": (_i, [_i, _i, _i, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz,
+                                         _vp]),
+    "qgemm_log_probabilities": (_i, [_i, _i, _vp, _sz, _vp, _i, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _vp]),
+    "qgemm_log_probabilities_backward": (_i, [_i, _i, _i, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp]),
     "qgemm_tile_map": (_i, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint32),
                             C.POINTER(C.c_uint32)]),
     "qgemm_quantize_grid": (_i, [_i, _sz, _sz, C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint32)]),

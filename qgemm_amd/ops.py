@@ -9,6 +9,10 @@
   layer_norm(x, ...), layer_norm_backward(dy, x, ...), checkpoint(x, ...), restore(q, scales, ...), weight_gradient(dy, q, scales, ...)
                                training around the products: a layer norm, activations kept in 8 bits, the gradients computed
                                from them (no counterpart in the reference)
+  rms_norm(x, ...), rms_norm_backward(dy, h, ...), group_rows(ids, ...), add_adapters(y, x, ...), add_adapters_backward(dy, x, ...),
+  log_probabilities(logits, tokens, ...), log_probabilities_backward(logits, tokens, ...)
+                               beside the products of a language model: its norm, low-rank adapters of many requests at once, what its
+                               last product says of tokens (no counterpart in the reference)
 
 Tensors are torch CUDA(HIP) tensors; only their data pointers and the current
 stream cross the boundary."""
@@ -34,7 +38,8 @@ _TORCH_DT = {
 
 _native_module = None
 _NATIVE_ENTRIES = ("ops_gemm", "ops_scaled_gemm", "ops_transpose", "ops_quantize", "ops_layer_norm", "ops_layer_norm_backward", "ops_checkpoint",
-                   "ops_restore", "ops_weight_gradient")
+                   "ops_restore", "ops_weight_gradient", "ops_rms_norm", "ops_rms_norm_backward", "ops_group_rows", "ops_add_adapters",
+                   "ops_add_adapters_backward", "ops_log_probabilities", "ops_log_probabilities_backward")
 
 
 def _native():
@@ -469,3 +474,251 @@ def weight_gradient(dy, q, scales, weight=None, bias=None, out_dtype=torch.float
     check(load_library().qgemm_weight_gradient(_dt(dy), _dt(q), _dt(dw), params, dy.data_ptr(), lddy, q.data_ptr(), ldq, s, w, b, dw.data_ptr(), cols,
                                                db.data_ptr(), rows, n, cols, _stream()))
     return dw, db
+
+
+# ---- beside the products of a language model.  Tensors are rows of their last dimension, as above; all of them on the current device.
+def _need_here(*ts):
+    _need_gpu(*ts)
+    here = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.device.index != here:
+            raise ValueError(f"tensors must be on the current device, cuda:{here}, got one on {t.device}")
+
+
+def _weight(weight, cols):
+    """(type, pointer) of a norm's weight, which may be None."""
+    params, w, _ = _parameters(weight, None, cols)
+    return params, w
+
+
+def _like(t, other, name, dtypes=None):
+    """ld of a tensor that has to have the rows of `other`, (rows, cols)."""
+    rows, cols, ld = _rows_of(t, name)
+    if (rows, cols) != other:
+        raise ValueError(f"{name} must be {other[0]} rows of {other[1]}, got shape {tuple(t.shape)}")
+    if dtypes is not None:
+        _need_type(t, dtypes, name)
+    return ld
+
+
+def rms_norm(x, weight=None, eps=1e-6, residual=None, out_dtype=None, codes=None, store_y=True):
+    """y, h, rstd = root-mean-square norm of the rows of x [..., cols], fp32 / bf16 / fp16: y = h * rstd * weight, rstd = 1 / sqrt(mean h^2 + eps), h = x, or with a
+    residual (x's shape) h = x + residual in the residual's type, the residual stream's next value; the norm is that of what h stores.  weight [cols] or
+    None.  y has x's type, or out_dtype; rstd is fp32.
+    codes (torch.int8 or torch.float8_e4m3fn): y, h, rstd, q, scales, where q and scales are y in 8 bits, as quantize(y, codes, QUANT_BLOCK_1x128) of the fp32 y
+    gives it: an operand of the block-scaled products.  store_y=False: y is None, and only its codes are written."""
+    native = _native()
+    if native:
+        st, *out = native.ops_rms_norm(x, weight, eps, residual, out_dtype, codes, store_y)
+        if st == 0:
+            return tuple(out) if codes is not None else tuple(out[:3])
+        if st > 0:
+            check(st)
+    _need_here(x, weight, residual)
+    rows, cols, ld = _rows_of(x, "x")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    _need_type(x, _FLOATS, "x")
+    _need_type(out_dtype, _FLOATS, "out_dtype")
+    params, w = _weight(weight, cols)
+    if not store_y and codes is None:
+        raise ValueError("nothing is asked for: neither y nor codes")
+    h, ldr = x, 0
+    if residual is not None:
+        ldr = _like(residual, (rows, cols), "residual", _FLOATS)
+        h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+    y = torch.empty(x.shape, dtype=out_dtype, device=x.device) if store_y else None
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    q = scales = None
+    if codes is not None:
+        _need_type(codes, _CODES, "codes")
+        q, scales = torch.empty(x.shape, dtype=codes, device=x.device), _scales_like(x, cols)
+    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    check(load_library().qgemm_rms_norm(
+        _dt(x), _dt(h), _TORCH_DT[out_dtype], params, DT_I8 if q is None else _dt(q), x.data_ptr(), ld, at(residual), ldr, w, eps,
+        None if residual is None else h.data_ptr(), cols, at(y), cols, rstd.data_ptr(), at(q), cols, at(scales), rows, cols, _stream()))
+    return (y, h, rstd) if codes is None else (y, h, rstd, q, scales)
+
+
+def rms_norm_backward(dy, h, rstd, weight=None, dh=None, out_dtype=None):
+    """dx, dweight of rms_norm: dy [..., cols], h and rstd as rms_norm gave them; dh: the gradient that arrives along the residual stream (of h), which is added: dx is
+    then the gradient of x and of the residual.  dx has dy's type, or out_dtype; dweight has weight's, and is None where weight is."""
+    native = _native()
+    if native:
+        st, *out = native.ops_rms_norm_backward(dy, h, rstd, weight, dh, out_dtype)
+        if st == 0:
+            return tuple(out)
+        if st > 0:
+            check(st)
+    _need_here(dy, h, rstd, weight, dh)
+    rows, cols, lddy = _rows_of(dy, "dy")
+    out_dtype = dy.dtype if out_dtype is None else out_dtype
+    _need_type(dy, _FLOATS, "dy")
+    _need_type(out_dtype, _FLOATS, "out_dtype")
+    ldh = _like(h, (rows, cols), "h", _FLOATS)
+    lddh = 0 if dh is None else _like(dh, (rows, cols), "dh", _FLOATS)
+    params, w = _weight(weight, cols)
+    r = _need_floats(rstd, rows, "rstd")
+    dx = torch.empty(dy.shape, dtype=out_dtype, device=dy.device)
+    dw = None if weight is None else torch.empty_like(weight)
+    check(load_library().qgemm_rms_norm_backward(
+        _dt(dy), _dt(h), DT_F32 if dh is None else _dt(dh), _dt(dx), params, dy.data_ptr(), lddy, h.data_ptr(), ldh, r, w, None if dh is None else dh.data_ptr(), lddh,
+        dx.data_ptr(), cols, None if dw is None else dw.data_ptr(), rows, cols, _stream()))
+    return dx, dw
+
+
+class RowGroups:
+    """Rows grouped by their adapters: what group_rows() gives and the adapters' products take.  `words` is the library's own."""
+    __slots__ = ("rows", "adapters", "words")
+
+    def __init__(self, rows, adapters, words):
+        self.rows, self.adapters, self.words = rows, adapters, words
+
+
+def group_rows(ids, adapters):
+    """RowGroups of the rows whose adapters are ids [rows], int32 or int64 on the device: 0 .. adapters - 1, any other number means none.  Made once, it serves every
+    add_adapters and add_adapters_backward whose rows have these adapters."""
+    native = _native()
+    if native:
+        st, words = native.ops_group_rows(ids, adapters)
+        if st == 0:
+            return RowGroups(ids.numel(), adapters, words)
+        if st > 0:
+            check(st)
+    _need_here(ids)
+    _need_type(ids, (torch.int32, torch.int64), "ids")
+    if not ids.is_contiguous():
+        raise ValueError(f"ids must be contiguous, got strides {ids.stride()}")
+    rows, n = ids.numel(), C.c_size_t()
+    check(load_library().qgemm_group_rows_words(rows, _size(adapters, "adapters"), C.byref(n)))
+    words = torch.empty(n.value, dtype=torch.int32, device=ids.device)
+    check(load_library().qgemm_group_rows(ids.element_size(), ids.data_ptr(), rows, adapters, words.data_ptr(), _stream()))
+    return RowGroups(rows, adapters, words)
+
+
+def _size(n, name):
+    if n < 0:
+        raise ValueError(f"{name} must not be negative, got {n}")
+    return n
+
+
+def _adapters(x, A, B, groups, scaling):
+    """rows, k, ldx, rank, n and the pointer of the scaling, of operands that fit together."""
+    if not isinstance(groups, RowGroups):
+        raise TypeError(f"groups must be what group_rows() gives, got {type(groups).__name__}")
+    _need_here(x, A, B, groups.words, scaling)
+    rows, k, ldx = _rows_of(x, "x")
+    _need_type(x, _FLOATS[1:], "x")
+    for t, name in ((A, "A"), (B, "B")):
+        _need_type(t, (x.dtype,), name)
+        if t.dim() != 3 or not t.is_contiguous() or min(t.shape) < 1:
+            raise ValueError(f"{name} must be contiguous [adapters, rank, columns], got shape {tuple(t.shape)} strides {t.stride()}")
+    if A.shape[0] != groups.adapters or A.shape[:2] != B.shape[:2] or A.shape[2] != k or rows != groups.rows:
+        raise ValueError(f"x {tuple(x.shape)}, A {tuple(A.shape)}, B {tuple(B.shape)} and groups of {groups.rows} rows and {groups.adapters} adapters do not fit together")
+    return rows, k, ldx, A.shape[1], B.shape[2], None if scaling is None else _need_floats(scaling, groups.adapters, "scaling")
+
+
+def add_adapters(y, x, A, B, groups, scaling=None, out=None, keep=False):
+    """out[t] = y[t] + scaling[i] * (x[t] A[i]^T) B[i] for every row t and its adapter i (group_rows); y[t] for a row of none.  x [..., k] bf16 or fp16; A [adapters, rank, k] and
+    B [adapters, rank, n] of x's type, the rank (up to 128) as rows of both; scaling [adapters] fp32 or None; y [..., n] is the result of the product that the adapters stand
+    beside, fp32 / bf16 / fp16.  out: a tensor like y, which may be y itself; None: a new one.
+    keep: out, u, where u [..., rank] fp32 is x A^T, what the backward pass needs."""
+    native = _native()
+    if native and isinstance(groups, RowGroups):
+        st, res, u = native.ops_add_adapters(y, x, A, B, groups.words, groups.rows, groups.adapters, scaling, out, keep)
+        if st == 0:
+            return (res, u) if keep else res
+        if st > 0:
+            check(st)
+    rows, k, ldx, rank, n, s = _adapters(x, A, B, groups, scaling)
+    _need_here(y, out)
+    ldy = _like(y, (rows, n), "y", _FLOATS)
+    if out is None:
+        out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    if out.shape != y.shape:
+        raise ValueError(f"out must have y's shape, {tuple(y.shape)}, got {tuple(out.shape)}")
+    ldo = _like(out, (rows, n), "out", (y.dtype,))
+    u = torch.empty((*x.shape[:-1], rank), dtype=torch.float32, device=x.device) if keep else None
+    check(load_library().qgemm_add_adapters(
+        _dt(x), _dt(y), y.data_ptr(), ldy, x.data_ptr(), ldx, A.data_ptr(), B.data_ptr(), s, groups.words.data_ptr(), out.data_ptr(), ldo,
+        None if u is None else u.data_ptr(), rows, groups.adapters, rank, k, n, _stream()))
+    return (out, u) if keep else out
+
+
+def add_adapters_backward(dy, x, u, A, B, groups, scaling=None, dx=None, grad_dtype=torch.float32):
+    """dx, dA, dB of add_adapters: dy [..., n] of x's type, u as add_adapters(..., keep=True) gave it.  dx: the gradient of x that arrives from the product beside the adapters, fp32 / bf16 /
+    fp16, to which theirs is added in a new tensor of its type; None: theirs alone, of x's type.  dA and dB have grad_dtype; zeros for adapters without rows.  (The gradient of
+    y is dy.)"""
+    native = _native()
+    if native and isinstance(groups, RowGroups):
+        st, *out = native.ops_add_adapters_backward(dy, x, u, A, B, groups.words, groups.rows, groups.adapters, scaling, dx, grad_dtype)
+        if st == 0:
+            return tuple(out)
+        if st > 0:
+            check(st)
+    rows, k, ldx, rank, n, s = _adapters(x, A, B, groups, scaling)
+    _need_here(dy, u, dx)
+    lddy = _like(dy, (rows, n), "dy", (x.dtype,))
+    _need_type(grad_dtype, _FLOATS, "grad_dtype")
+    up = _need_floats(u, rows * rank, "u")
+    ld0 = k if dx is None else _like(dx, (rows, k), "dx", _FLOATS)
+    res = torch.empty(x.shape, dtype=x.dtype if dx is None else dx.dtype, device=x.device)
+    dA, dB = (torch.empty(t.shape, dtype=grad_dtype, device=x.device) for t in (A, B))
+    check(load_library().qgemm_add_adapters_backward(
+        _dt(x), _dt(res), _dt(dA), dy.data_ptr(), lddy, x.data_ptr(), ldx, up, A.data_ptr(), B.data_ptr(), s, groups.words.data_ptr(),
+        None if dx is None else dx.data_ptr(), ld0, res.data_ptr(), k, dA.data_ptr(), dB.data_ptr(), rows, groups.adapters, rank, k, n, _stream()))
+    return res, dA, dB
+
+
+def _tokens(tokens, rows):
+    _need_here(tokens)
+    _need_type(tokens, (torch.int32, torch.int64), "tokens")
+    if tokens.numel() != rows or not tokens.is_contiguous():
+        raise ValueError(f"tokens must hold {rows} contiguous numbers, got shape {tuple(tokens.shape)}")
+    return tokens.data_ptr()
+
+
+def log_probabilities(logits, tokens, top=0):
+    """logp, entropy, lse [...] fp32 of logits [..., vocabulary], fp32 / bf16 / fp16, and tokens [...], int32 or int64: log softmax at the token, the softmax's entropy, log sum
+    exp.  A token outside the vocabulary (-100) asks for nothing, its logp is 0.  -inf is a token that cannot be; a row of nothing else has lse = logp = -inf
+    and entropy 0.
+    top (up to 32): logp, entropy, lse, values, indices [..., top], the most probable tokens (int64) and their log probabilities, equal ones in the order of their numbers."""
+    native = _native()
+    if native:
+        st, *out = native.ops_log_probabilities(logits, tokens, top)
+        if st == 0:
+            return tuple(out) if top else tuple(out[:3])
+        if st > 0:
+            check(st)
+    _need_here(logits)
+    rows, cols, ld = _rows_of(logits, "logits")
+    _need_type(logits, _FLOATS, "logits")
+    t = _tokens(tokens, rows)
+    lead = logits.shape[:-1]
+    logp, entropy, lse = (torch.empty(lead, dtype=torch.float32, device=logits.device) for _ in range(3))
+    values, indices = (torch.empty((*lead, _size(top, "top")), dtype=d, device=logits.device) for d in (torch.float32, torch.int64))
+    check(load_library().qgemm_log_probabilities(_dt(logits), tokens.element_size(), logits.data_ptr(), ld, t, top, logp.data_ptr(), entropy.data_ptr(),
+                                                 lse.data_ptr(), values.data_ptr(), indices.data_ptr(), rows, cols, _stream()))
+    return (logp, entropy, lse, values, indices) if top else (logp, entropy, lse)
+
+
+def log_probabilities_backward(logits, tokens, lse, entropy, dlogp, dentropy=None, out_dtype=None):
+    """dlogits = dlogp * ([token] - p) - dentropy * p * (log p + entropy), of logits' type or out_dtype: the gradient of the logits out of those of log_probabilities' logp and
+    entropy (None: zeros); lse and entropy as it gave them."""
+    native = _native()
+    if native:
+        st, out = native.ops_log_probabilities_backward(logits, tokens, lse, entropy, dlogp, dentropy, out_dtype)
+        if st == 0:
+            return out
+        if st > 0:
+            check(st)
+    _need_here(logits, lse, entropy, dlogp, dentropy)
+    rows, cols, ld = _rows_of(logits, "logits")
+    out_dtype = logits.dtype if out_dtype is None else out_dtype
+    _need_type(logits, _FLOATS, "logits")
+    _need_type(out_dtype, _FLOATS, "out_dtype")
+    t = _tokens(tokens, rows)
+    at = [None if v is None else _need_floats(v, rows, name) for v, name in ((lse, "lse"), (entropy, "entropy"), (dlogp, "dlogp"), (dentropy, "dentropy"))]
+    out = torch.empty(logits.shape, dtype=out_dtype, device=logits.device)
+    check(load_library().qgemm_log_probabilities_backward(_dt(logits), _dt(out), tokens.element_size(), logits.data_ptr(), ld, t, *at, out.data_ptr(), cols, rows, cols,
+                                                          _stream()))
+    return out
