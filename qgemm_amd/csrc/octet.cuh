@@ -34,6 +34,7 @@ __device__ __forceinline__ bool any_repeated(uint32_t c, uint32_t cols) {
 }
 template <int DT>
 struct Octet {
+    static constexpr int TYPE = DT;
     static constexpr int ES = DT == QGEMM_DT_F32 ? 4 : (DT == QGEMM_DT_BF16 || DT == QGEMM_DT_F16) ? 2 : 1, DW = 2 * ES;
     uint32_t w[DW];
 
@@ -101,6 +102,28 @@ struct Octet {
                 v[4 * i] = lo[0], v[4 * i + 1] = lo[1], v[4 * i + 2] = hi[0], v[4 * i + 3] = hi[1];
             }
         }
+    }
+    // eight numbers, rounded to nearest even where the type has fewer bits (fp32, bf16 and fp16)
+    __device__ __forceinline__ void take(const float (&v)[8]) {
+        if constexpr (DT == QGEMM_DT_F32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __builtin_bit_cast(uint32_t, v[i]);
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const v2i p = DT == QGEMM_DT_BF16 ? pack4_bf16(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3])
+                                                  : pack4_f16(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+                w[2 * h] = (uint32_t)p[0], w[2 * h + 1] = (uint32_t)p[1];
+            }
+        }
+    }
+    // as elements of a row of eight or more (c < cols; rows that are no ROW_ANY)
+    template <int ROW>
+    __device__ __forceinline__ void put(void *row, uint32_t c, uint32_t cols) const {
+        static_assert(ROW != ROW_ANY, "rows of eight elements and more");
+        char *at = (char *)row + (row_offset<ROW>)octet_begin<ROW>(c, cols) * ES;
+#pragma unroll
+        for (int i = 0; i < DW / 4; ++i) *(v4i_any *)(at + 16 * i) = v4i{(int)w[4 * i], (int)w[4 * i + 1], (int)w[4 * i + 2], (int)w[4 * i + 3]};
     }
 
 private:

@@ -53,6 +53,43 @@ __device__ __forceinline__ void quantize_octet(const RmsArgs &p, uint32_t row, u
     if (c % kScaleBlock == 0) p.scales[(size_t)row * p.kb + c / kScaleBlock] = scale;
 }
 
+// A lane's octets of the weight, of any type, as they come from memory (ones where there is none), and as numbers.  (Registers for fp32, and one branch for all
+// octets: the kernels would be twice as many with the weight's type among their own.)
+template <int TYPE, int P, int ROW, class Args>
+__device__ __forceinline__ void weight_octets(const Args &p, uint32_t first, uint32_t step, uint32_t (&w)[P][8]) {
+    Octet<TYPE> all[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) all[i].template request<ROW>(p.weight, first + i * step, p.cols);
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[i][k] = k < Octet<TYPE>::DW ? all[i].w[k % Octet<TYPE>::DW] : 0;
+}
+// columns first + i step
+template <int P, int ROW, class Args>
+__device__ __forceinline__ void weight_request(const Args &p, uint32_t first, uint32_t step, uint32_t (&w)[P][8]) {
+    if (!p.weight) {
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[i][k] = 0x3F800000u;
+    } else if (p.param_dt == QGEMM_DT_F32) {
+        weight_octets<QGEMM_DT_F32, P, ROW>(p, first, step, w);
+    } else {
+        weight_octets<QGEMM_DT_BF16, P, ROW>(p, first, step, w);          // (16 bits, whichever)
+    }
+}
+template <class Args>
+__device__ __forceinline__ void weight_floats(const Args &p, const uint32_t (&w)[8], float (&f)[8]) {
+    const bool wide = !p.weight || p.param_dt == QGEMM_DT_F32, bf16 = p.param_dt == QGEMM_DT_BF16;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t half = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu;
+        const float narrow = bf16 ? __builtin_bit_cast(float, half << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)half);
+        f[e] = wide ? __builtin_bit_cast(float, w[e]) : narrow;
+    }
+}
+
 // ---- rows of any length: a workgroup goes over its row twice, the second time out of the caches
 __global__ void __launch_bounds__(256) rms_any_kernel(const RmsArgs p) {
     __shared__ float red[2][4][1];
@@ -95,6 +132,84 @@ __global__ void __launch_bounds__(256) rms_any_kernel(const RmsArgs p) {
     }
 }
 
+// ---- rows in registers: GROUP threads hold a row, P octets each, and read x and the residual once.  RES: type of the residual, -1 where there is none.
+// Bound by memory: 6144 x 7168 bf16 with residual, y and int8 codes 80 us in a trace, 4.95 TB/s, the rate of a copy; 107 in two passes out of the caches
+// (rms_any_kernel).  1 x 7168: 5.5, a trip to memory, a barrier, the division by the scale and the stores.
+template <int DT, int RES, int GROUP, int P, int ROW>
+__global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) rms_rows_kernel(const RmsArgs p) {
+    constexpr int THREADS = GROUP < 256 ? 256 : GROUP, ROWS = THREADS / GROUP, WAVES = GROUP / 64, LANES = GROUP < 64 ? GROUP : 64;
+    constexpr int H_DT = RES < 0 ? DT : RES;
+    const uint32_t t = threadIdx.x % GROUP, cols = p.cols;
+    auto column = [&](int i) { return (i * GROUP + t) * kOctet; };
+    int turn = 0;
+    for (uint32_t first = blockIdx.x * ROWS; first < p.rows; first += gridDim.x * ROWS, turn ^= 1) {
+        const uint32_t row = ROWS == 1 ? first : first + threadIdx.x / GROUP;
+        const bool in_rows = ROWS == 1 || row < p.rows;
+        const size_t at = in_rows ? row : p.rows - 1;
+        Octet<DT> x[P];
+        Octet<H_DT> h[P];
+        uint32_t w[P][8];
+        const char *xr = (const char *)p.x + at * p.ldx * Octet<DT>::ES, *rr = (const char *)p.residual + at * p.ldr * Octet<H_DT>::ES;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            x[i].template request<ROW>(xr, column(i), cols);
+            if constexpr (RES >= 0) h[i].template request<ROW>(rr, column(i), cols);
+        }
+        weight_request<P, ROW>(p, t * kOctet, GROUP * kOctet, w);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float v[8];
+            x[i].template settle<ROW>(column(i), cols);
+            x[i].floats(v);
+            if constexpr (RES >= 0) {
+                float r[8];
+                h[i].template settle<ROW>(column(i), cols);
+                h[i].floats(r);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += r[e];
+                h[i].take(v);
+                h[i].hold();
+                h[i].floats(v);
+                if (in_rows && column(i) < cols)
+                    h[i].template put<ROW>((char *)p.h + at * p.ldh * Octet<H_DT>::ES, column(i), cols);
+            } else {
+                h[i] = x[i];
+                h[i].hold();
+            }
+            if (any_repeated<ROW>(column(i), cols))
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = e < (int)repeated<ROW>(column(i), cols) ? 0.0f : v[e];
+            sum += ((v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3])) + ((v[4] * v[4] + v[5] * v[5]) + (v[6] * v[6] + v[7] * v[7]));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        sum = lanes_sum<LANES>(sum);
+        if constexpr (WAVES > 1) {
+            __shared__ float red[2][WAVES];
+            if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = sum;
+            __syncthreads();
+            sum = red[turn][0];
+#pragma unroll
+            for (int i = 1; i < WAVES; ++i) sum += red[turn][i];
+        }
+        const float rstd = 1.0f / __builtin_sqrtf(sum / (float)cols + p.eps);
+        if (t == 0 && in_rows && p.rstd) p.rstd[row] = rstd;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const uint32_t c = column(i);
+            float v[8], f[8];
+            h[i].hold();
+            h[i].floats(v);
+            weight_floats(p, w[i], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = c < cols ? v[e] * rstd * f[e] : 0.0f;
+            if (p.q && in_rows) quantize_octet<ROW>(p, row, c, v);
+            if (p.y && in_rows && c < cols) store_octet<ROW>((char *)p.y + at * p.ldy * dtype_bytes(p.y_dt), p.y_dt, c, cols, v);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+}
+
 // ---- backward
 // rows of any length: sums of a row, then its dx, out of the caches
 __global__ void __launch_bounds__(256) rms_backward_any_kernel(const RmsBackwardArgs p) {
@@ -133,6 +248,143 @@ __global__ void __launch_bounds__(256) rms_backward_any_kernel(const RmsBackward
                 for (int e = 0; e < 8; ++e) g[e] += xhat[e];
             }
             store_octet((char *)p.dx + (size_t)row * p.lddx * dtype_bytes(p.dx_dt), p.dx_dt, c, p.cols, g);
+        }
+    }
+}
+
+// Rows in registers: GROUP threads hold a row of dy and of h, P octets each; a workgroup goes over its rows with the next one's loads in flight, and
+// keeps the sums of its columns in registers until the end.  S_DT: type of h and dh; DH: there is a dh, which is wanted at the end of a row's work
+// and requested at its beginning.  Bound by memory: 8192 x 4096 bf16 with dh 42 us, 6.4 TB/s, part of it out of the last-level cache, and 4.5 for the workgroups'
+// sums; 77 in two passes over the rows and one for the columns.  1999 x 3001 fp16 13.7 with both launches, 25 before: four rows a workgroup, one in flight.
+template <int DY_DT, int S_DT, bool DH, int GROUP, int P, int ROW>
+__global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) rms_backward_rows_kernel(const RmsBackwardArgs p) {
+    constexpr int THREADS = GROUP < 256 ? 256 : GROUP, ROWS = THREADS / GROUP, WAVES = GROUP / 64, LANES = GROUP < 64 ? GROUP : 64;
+    const uint32_t t = threadIdx.x % GROUP, sub = ROWS == 1 ? 0 : threadIdx.x / GROUP, cols = p.cols;
+    auto column = [&](int i) { return (i * GROUP + t) * kOctet; };
+    struct Row {
+        Octet<DY_DT> dy[P];
+        Octet<S_DT> h[P];
+        float rstd;
+    };
+    auto row_of = [&](uint32_t first) {
+        const uint32_t row = first + sub;
+        return ROWS == 1 || row < p.rows ? row : p.rows - 1;
+    };
+    auto fetch = [&](Row &r, uint32_t first) {
+        const size_t row = row_of(first);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            r.dy[i].template request<ROW>((const char *)p.dy + row * p.lddy * Octet<DY_DT>::ES, column(i), cols);
+            r.h[i].template request<ROW>((const char *)p.h + row * p.ldh * Octet<S_DT>::ES, column(i), cols);
+        }
+        r.rstd = p.rstd[row];
+    };
+    float w[P][8], dw[P][8] = {};
+    {
+        uint32_t bits[P][8];
+        weight_request<P, ROW>(p, t * kOctet, GROUP * kOctet, bits);
+#pragma unroll
+        for (int i = 0; i < P; ++i) weight_floats(p, bits[i], w[i]);
+    }
+    Row next;
+    const uint32_t stride = gridDim.x * ROWS;
+    fetch(next, blockIdx.x * ROWS);
+    int turn = 0;
+    for (uint32_t first = blockIdx.x * ROWS; first < p.rows; first += stride, turn ^= 1) {
+        Row r = next;
+        const bool in_rows = ROWS == 1 || first + sub < p.rows;
+        Octet<S_DT> dh[DH ? P : 1];
+        if constexpr (DH)
+#pragma unroll
+            for (int i = 0; i < P; ++i) dh[i].template request<ROW>((const char *)p.dh + (size_t)row_of(first) * p.lddh * Octet<S_DT>::ES, column(i), cols);
+        if (p.rows - first > stride) fetch(next, first + stride);
+        float b = 0.0f;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float g[8], xhat[8];
+            r.dy[i].template settle<ROW>(in_rows ? column(i) : cols, cols);
+            r.h[i].template settle<ROW>(column(i), cols);
+            r.dy[i].hold();
+            r.h[i].hold();
+            r.dy[i].floats(g);
+            r.h[i].floats(xhat);
+            const float by = column(i) < cols ? r.rstd : 0.0f;      // (0 times an infinite rstd is no 0)
+            if (any_repeated<ROW>(column(i), cols))
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[e] = e < (int)repeated<ROW>(column(i), cols) ? 0.0f : g[e];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float product = g[e] * (xhat[e] * by);
+                dw[i][e] += product;
+                b += product * w[i][e];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        b = lanes_sum<LANES>(b);
+        if constexpr (WAVES > 1) {
+            __shared__ float red[2][WAVES];
+            if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = b;
+            __syncthreads();
+            b = red[turn][0];
+#pragma unroll
+            for (int i = 1; i < WAVES; ++i) b += red[turn][i];
+        }
+        b /= (float)cols;
+        char *dx = (char *)p.dx + (size_t)(first + sub) * p.lddx * dtype_bytes(p.dx_dt);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float g[8], xhat[8];
+            r.dy[i].hold();
+            r.h[i].hold();
+            r.dy[i].floats(g);
+            r.h[i].floats(xhat);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[e] = r.rstd * (g[e] * w[i][e] - xhat[e] * r.rstd * b);
+            if constexpr (DH) {
+                float more[8];
+                dh[i].template settle<ROW>(column(i), cols);
+                dh[i].floats(more);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[e] += more[e];
+            }
+            if (in_rows && column(i) < cols) store_octet<ROW>(dx, p.dx_dt, column(i), cols, g);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    if (!p.dweight) return;
+    float *out = p.partial + (size_t)blockIdx.x * norm_partial_cols(cols);
+    if constexpr (ROWS == 1) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if (column(i) >= cols) continue;
+            if (const uint32_t before = repeated<ROW>(column(i), cols)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e >= (int)before) out[column(i) - before + e] = dw[i][e];
+                continue;
+            }
+            v4f *at = (v4f *)(out + column(i));
+            at[0] = v4f{dw[i][0], dw[i][1], dw[i][2], dw[i][3]};
+            at[1] = v4f{dw[i][4], dw[i][5], dw[i][6], dw[i][7]};
+        }
+    } else {
+        __shared__ float fold[THREADS * 8];                     // [ROWS][GROUP * 8]
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int before = (int)repeated<ROW>(column(i), cols);
+                if (ROW != ROW_RAGGED || e >= before) fold[threadIdx.x * 8 + e - before] = dw[i][e];
+            }
+            __syncthreads();
+#pragma unroll 1
+            for (uint32_t c = threadIdx.x; c < GROUP * 8; c += THREADS) {
+                float s = fold[c];
+#pragma unroll
+                for (int k = 1; k < ROWS; ++k) s += fold[k * GROUP * 8 + c];
+                if (i * GROUP * 8 + c < cols) out[i * GROUP * 8 + c] = s;
+            }
         }
     }
 }
