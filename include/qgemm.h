@@ -244,7 +244,7 @@ int qgemm_rms_norm_backward(int dy_dtype, int h_dtype, int dh_dtype, int dx_dtyp
 
 /* Rows grouped by the adapter that each of them has, once for all calls below with the same ids.
  *   ids      rows integers of id_bytes 4 or 8: 0 .. adapters - 1; any other number means no adapter
- *   groups   device memory of qgemm_group_rows_words 32-bit words, 8-byte aligned; its contents are the library's own
+ *   groups   device memory of qgemm_group_rows_words 32-bit words, 16-byte aligned; its contents are the library's own
  * Up to 65535 adapters and 2^28 - 1 rows. */
 int qgemm_group_rows_words(size_t rows, size_t adapters, size_t *words);
 int qgemm_group_rows(int id_bytes, const void *ids, size_t rows, size_t adapters, void *groups, void *stream);
@@ -256,7 +256,7 @@ int qgemm_group_rows(int id_bytes, const void *ids, size_t rows, size_t adapters
  *   scaling   adapters floats, or NULL: 1
  *   groups    of these rows and this number of adapters
  *   u         A[i] x[t] for the backward pass, rows x rank floats (zeros for rows of no adapter), or NULL
- * A[i] x[t] has fp32 accumulators and goes on in 16 bits of mantissa, in 24 where y is F32.  Uses the library workspace.  Up to 2^24 - 256 columns. */
+ * A[i] x[t] has fp32 accumulators and goes on in 16 bits of mantissa, in 24 where y is F32.  Uses the library workspace.  Up to 2^23 - 256 columns. */
 int qgemm_add_adapters(int dtype, int y_dtype, const void *y, size_t ldy, const void *x, size_t ldx, const void *A, const void *B,
                        const float *scaling, const void *groups, void *out, size_t ldo, float *u, size_t rows, size_t adapters,
                        size_t rank, size_t k, size_t n, void *stream);

@@ -60,14 +60,15 @@ struct RowGroups {
     const int32_t *order;                // rows, group by group, in their own order within a group
     const int32_t *offsets;              // where group i starts in `order`: adapters + 2, the last being the number of rows
     const int32_t *first;                // first slot of group i: adapters + 1
-    const v2i *slots;                    // group of a slot, -1 for none, and where it starts in `order`
+    const v4i *slots;                    // group of a slot (-1: none), where it starts in `order`, its rows, its number in the group
     uint32_t rows, adapters, slot_count;
 };
 inline size_t group_slots(size_t rows, size_t adapters) { return rows / kSlotRows + (rows < adapters + 1 ? rows : adapters + 1); }
-inline size_t group_words(size_t rows, size_t adapters) { return (rows + 2 * adapters + 4) / 2 * 2 + 2 * group_slots(rows, adapters); }
+inline size_t group_slots_at(size_t rows, size_t adapters) { return (rows + 2 * adapters + 3 + 3) / 4 * 4; }
+inline size_t group_words(size_t rows, size_t adapters) { return group_slots_at(rows, adapters) + 4 * group_slots(rows, adapters); }
 inline RowGroups row_groups(const void *words, size_t rows, size_t adapters) {
     const int32_t *w = (const int32_t *)words;
-    return RowGroups{w, w + rows, w + rows + adapters + 2, (const v2i *)(w + (rows + 2 * adapters + 4) / 2 * 2), (uint32_t)rows, (uint32_t)adapters,
+    return RowGroups{w, w + rows, w + rows + adapters + 2, (const v4i *)(w + group_slots_at(rows, adapters)), (uint32_t)rows, (uint32_t)adapters,
                      (uint32_t)group_slots(rows, adapters)};
 }
 hipError_t launch_group_rows(const void *ids, int id_bytes, const RowGroups &g, hipStream_t stream);
@@ -88,7 +89,7 @@ struct ShrinkArgs {                      // u[row] = W[its adapter] x[row]
     uint32_t cols, rank, part;           // part: columns of a split
     int dt, zero;                        // zero: rows without an adapter get zeros
 };
-uint32_t plan_shrink(const ShrinkArgs &a, int cus);       // splits
+void plan_shrink(ShrinkArgs &a, int cus);                 // chooses u.planes and part
 hipError_t launch_shrink(const ShrinkArgs &a, hipStream_t stream);
 
 struct ExpandArgs {                      // out[row] = y[row] + scaling[its adapter] u[row] W[its adapter]; y null: zeros
@@ -99,23 +100,29 @@ struct ExpandArgs {                      // out[row] = y[row] + scaling[its adap
     float *keep;                         // u's parts added up, [rows][rank], or null
     RankSums u;
     uint64_t ldy, ldo;
-    uint32_t cols, rank;
+    uint32_t cols, rank, wide;           // wide: columns of a workgroup
     int dt, y_dt;
 };
-hipError_t launch_expand(const ExpandArgs &a, hipStream_t stream);
+hipError_t launch_expand(ExpandArgs a, int cus, hipStream_t stream);
 
-struct AdapterGradArgs {                 // dw[i] = scaling[i] sum over the rows of adapter i of u[row] z[row]^T
-    RowGroups g;
+// dw[i] = scaling[i] sum over the rows of adapter i of u[row] z[row]^T, of up to two factors in one launch
+struct AdapterGrad {
     const void *z;
-    const float *scaling;
-    void *dw;                            // [adapters][rank][cols]
+    void *dw;                            // [adapters][rank][cols]; null: not wanted
     float *room;                         // parts of groups of more than `chunk` slots
     RankSums u;
     uint64_t ldz;
-    uint32_t cols, rank, chunk;
+    uint32_t cols;
+};
+struct AdapterGradArgs {
+    RowGroups g;
+    AdapterGrad of[2];
+    const float *scaling;
+    uint32_t rank, chunk, tiles;         // tiles: column tiles of the first factor
     int dt, dw_dt;
 };
-size_t plan_adapter_grad(AdapterGradArgs &a, int cus);    // chooses chunk; bytes of `room`
+size_t plan_adapter_grad(AdapterGradArgs &a, int cus);    // chooses chunk; bytes of both rooms, one behind the other
+void place_adapter_grad(AdapterGradArgs &a, float *room);
 hipError_t launch_adapter_grad(const AdapterGradArgs &a, hipStream_t stream);
 
 }  // namespace qgemm

@@ -1829,7 +1829,7 @@ int keep_entry(bool encode, int in_dt, int out_dt, const void *in, size_t ld_in,
 int adapters_size_status(size_t rows, size_t adapters, size_t rank, size_t k, size_t n) {
     if (adapters == 0 || rank == 0 || k == 0 || n == 0) return QGEMM_ERR_INVALID_ARG;
     if (rows >= ((size_t)1 << 28) || adapters > kMostAdapters || rank > kMostRank) return QGEMM_ERR_TOO_LARGE;
-    if (k > (size_t)kMaxGridY * 256 || n > (size_t)kMaxGridY * 256) return QGEMM_ERR_TOO_LARGE;       // (columns are the y extent of launches)
+    if (k > ((size_t)1 << 23) - 256 || n > ((size_t)1 << 23) - 256) return QGEMM_ERR_TOO_LARGE;       // (the columns of both are the y extent of a launch)
     return QGEMM_OK;
 }
 ShrinkArgs shrink_args(int dtype, const void *groups, const void *x, size_t ldx, const void *w, size_t rows, size_t adapters, size_t rank, size_t cols) {
@@ -1845,9 +1845,7 @@ ShrinkArgs shrink_args(int dtype, const void *groups, const void *x, size_t ldx,
 // Where the sums over the rank go: `u`, [rows][rank], where the caller wants them and they come in one part, else into the workspace, of
 // which the bytes are returned
 size_t plan_rank_sums(ShrinkArgs &s, float *u) {
-    s.u.planes = plan_shrink(s, g_ctx.num_cus);
-    s.part = (uint32_t)(((s.cols + s.u.planes - 1) / s.u.planes + 255) / 256 * 256);
-    s.u.planes = (s.cols + s.part - 1) / s.part;
+    plan_shrink(s, g_ctx.num_cus);
     if (u && s.u.planes == 1) {
         s.u.at = u;
         s.u.pitch = s.rank;
@@ -2315,7 +2313,7 @@ QGEMM_EXPORT int qgemm_group_rows(int id_bytes, const void *ids, size_t rows, si
     if (id_bytes != 4 && id_bytes != 8) return QGEMM_ERR_UNSUPPORTED;
     if (adapters == 0) return QGEMM_ERR_INVALID_ARG;
     if (rows >= ((size_t)1 << 28) || adapters > kMostAdapters) return QGEMM_ERR_TOO_LARGE;
-    if (!groups || (uintptr_t)groups % 8 || (rows && !ids)) return QGEMM_ERR_INVALID_ARG;
+    if (!groups || (uintptr_t)groups % 16 || (rows && !ids)) return QGEMM_ERR_INVALID_ARG;
     std::lock_guard<std::mutex> lock(g_ctx.mu);
     const int st = ensure_init_locked();
     if (st != QGEMM_OK) return st;
@@ -2330,7 +2328,7 @@ QGEMM_EXPORT int qgemm_add_adapters(int dtype, int y_dtype, const void *y, size_
     int st = adapters_size_status(rows, adapters, rank, k, n);
     if (st != QGEMM_OK) return st;
     if (rows == 0) return QGEMM_OK;
-    if (!y || !x || !A || !B || !groups || (uintptr_t)groups % 8 || !out || ldy < n || ldx < k || ldo < n || (out == y && ldo != ldy)) return QGEMM_ERR_INVALID_ARG;
+    if (!y || !x || !A || !B || !groups || (uintptr_t)groups % 16 || !out || ldy < n || ldx < k || ldo < n || (out == y && ldo != ldy)) return QGEMM_ERR_INVALID_ARG;
     hipStream_t stream = (hipStream_t)stream_;
     std::lock_guard<std::mutex> lock(g_ctx.mu);
     st = ensure_init_locked();
@@ -2348,7 +2346,7 @@ QGEMM_EXPORT int qgemm_add_adapters(int dtype, int y_dtype, const void *y, size_
     e.keep = room ? u : nullptr;
     g_ctx.last_config = "add_adapters";
     if (launch_shrink(s, stream) != hipSuccess) return QGEMM_ERR_LAUNCH;
-    return launch_expand(e, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+    return launch_expand(e, g_ctx.num_cus, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
 }
 
 QGEMM_EXPORT int qgemm_add_adapters_backward(int dtype, int dx_dtype, int grad_dtype, const void *dy, size_t lddy, const void *x, size_t ldx, const float *u,
@@ -2359,7 +2357,7 @@ QGEMM_EXPORT int qgemm_add_adapters_backward(int dtype, int dx_dtype, int grad_d
     int st = adapters_size_status(rows, adapters, rank, k, n);
     if (st != QGEMM_OK) return st;
     if (rows == 0 && !dA && !dB) return QGEMM_OK;
-    if (!groups || (uintptr_t)groups % 8) return QGEMM_ERR_INVALID_ARG;
+    if (!groups || (uintptr_t)groups % 16) return QGEMM_ERR_INVALID_ARG;
     if (rows && (!dy || !x || !A || !B || lddy < n || ldx < k || (dB && !u) || (dx0 && !dx) || (dx && lddx < k) || (dx0 && lddx0 < k) ||
                  (dx0 && dx0 == dx && lddx0 != lddx)))
         return QGEMM_ERR_INVALID_ARG;
@@ -2369,32 +2367,38 @@ QGEMM_EXPORT int qgemm_add_adapters_backward(int dtype, int dx_dtype, int grad_d
     if (st != QGEMM_OK) return st;
     WorkspaceUse ws_use(stream);
     ShrinkArgs s = shrink_args(dtype, groups, dy, lddy, B, rows, adapters, rank, n);
-    const size_t sums = rows && (dx || dA) ? (plan_rank_sums(s, nullptr) + 255) / 256 * 256 : 0;
-    auto gradient = [&](const void *z, size_t ldz, size_t cols, RankSums of, void *dw) {
-        AdapterGradArgs g;
-        std::memset(&g, 0, sizeof(g));
-        g.g = s.g;
-        g.z = z, g.scaling = scaling, g.dw = dw;
-        g.u = of;
-        g.ldz = ldz;
-        g.cols = (uint32_t)cols, g.rank = (uint32_t)rank;
-        g.dt = dtype, g.dw_dt = grad_dtype;
-        return g;
-    };
-    AdapterGradArgs ga = gradient(x, ldx, k, s.u, dA), gb = gradient(dy, lddy, n, RankSums{const_cast<float *>(u), 0, (uint32_t)rank, 1}, dB);
-    const size_t room = std::max(dA ? plan_adapter_grad(ga, g_ctx.num_cus) : 0, dB ? plan_adapter_grad(gb, g_ctx.num_cus) : 0);
-    if (sums + room) {
-        void *ws = nullptr;
-        st = ensure_workspace_locked(sums + room, stream, &ws);
+    auto whole = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
+    const size_t sums = rows && (dx || dA) ? whole(plan_rank_sums(s, nullptr)) : 0;
+    // (parts of v are added up once, where dx is computed, for all columns of dA)
+    const size_t joined = dx && dA && s.u.planes > 1 ? whole(rows * rank * sizeof(float)) : 0;
+    AdapterGradArgs g;
+    std::memset(&g, 0, sizeof(g));
+    g.g = s.g;
+    g.scaling = scaling;
+    g.rank = (uint32_t)rank;
+    g.dt = dtype, g.dw_dt = grad_dtype;
+    g.of[0].z = x, g.of[0].dw = dA, g.of[0].ldz = ldx, g.of[0].cols = (uint32_t)k, g.of[0].u = s.u;
+    g.of[1].z = dy, g.of[1].dw = dB, g.of[1].ldz = lddy, g.of[1].cols = (uint32_t)n;
+    g.of[1].u = RankSums{const_cast<float *>(u), 0, (uint32_t)rank, 1};
+    const size_t room = dA || dB ? plan_adapter_grad(g, g_ctx.num_cus) : 0;
+    void *ws = nullptr;
+    if (sums + joined + room) {
+        st = ensure_workspace_locked(sums + joined + room, stream, &ws);
         if (st != QGEMM_OK) return st;
-        s.u.at = ga.u.at = (float *)ws;
-        ga.room = gb.room = (float *)((char *)ws + sums);
+        s.u.at = (float *)ws;
+        float *v = (float *)((char *)ws + sums);
+        g.of[0].u = joined ? RankSums{v, 0, (uint32_t)rank, 1} : s.u;
+        place_adapter_grad(g, (float *)((char *)ws + sums + joined));
     }
     g_ctx.last_config = "add_adapters_backward";
     if (sums && launch_shrink(s, stream) != hipSuccess) return QGEMM_ERR_LAUNCH;
-    if (rows && dx && launch_expand(expand_args(s, dx_dtype, A, scaling, dx0, dx0 ? lddx0 : lddx, dx, lddx, k), stream) != hipSuccess) return QGEMM_ERR_LAUNCH;
-    if (dA && launch_adapter_grad(ga, stream) != hipSuccess) return QGEMM_ERR_LAUNCH;
-    return !dB || launch_adapter_grad(gb, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+    if (rows && dx) {
+        ExpandArgs e = expand_args(s, dx_dtype, A, scaling, dx0, dx0 ? lddx0 : lddx, dx, lddx, k);
+        e.keep = joined ? (float *)((char *)ws + sums) : nullptr;
+        if (launch_expand(e, g_ctx.num_cus, stream) != hipSuccess) return QGEMM_ERR_LAUNCH;
+    }
+    if (!dA && !dB) return QGEMM_OK;
+    return launch_adapter_grad(g, stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
 }
 
 QGEMM_EXPORT int qgemm_log_probabilities(int dtype, int token_bytes, const void *logits, size_t ld, const void *tokens, int top, float *logp, float *entropy,

@@ -87,12 +87,12 @@ def test_groups(rows, adapters, kind, dtype):
     offsets = np.concatenate([[0], np.cumsum(counts)])
     assert np.array_equal(w[rows:rows + adapters + 2], offsets)
     first = w[rows + adapters + 2:rows + 2 * adapters + 3]
-    slots = w[(rows + 2 * adapters + 4) // 2 * 2:].reshape(-1, 2)
+    slots = w[(rows + 2 * adapters + 6) // 4 * 4:].reshape(-1, 4)
     assert len(slots) == rows // 64 + min(rows, adapters + 1)
     want = {}
     for a in np.nonzero(counts)[0]:
         for j in range(-(-counts[a] // 64)):
-            want[int(first[a]) + j] = (int(a), int(offsets[a]) + 64 * j)
+            want[int(first[a]) + j] = (int(a), int(offsets[a]) + 64 * j, int(min(64, counts[a] - 64 * j)), j)
     assert {i: tuple(map(int, s)) for i, s in enumerate(slots) if s[0] >= 0} == want
 
 

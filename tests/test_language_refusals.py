@@ -51,16 +51,16 @@ def log_prob_backward(dt=BF16, out=BF16, bytes=8, x=P, ld=64, t=P, lse=P, entrop
     (norm_backward, INVALID, [dict(dy=None), dict(h=None), dict(dx=None), dict(rstd=None), dict(cols=0), dict(lddy=63), dict(ldh=63), dict(lddh=63), dict(lddx=63)]),
     (norm_backward, TOO_LARGE, [dict(rows=1 << 31), dict(cols=1 << 31), dict(cols=(1 << 31) - 1, lddy=1 << 31, ldh=1 << 31, lddh=1 << 31, lddx=1 << 31)]),
     (group, UNSUPPORTED, [dict(bytes=2)]),
-    (group, INVALID, [dict(ids=None), dict(adapters=0), dict(groups=None), dict(groups=P + 4)]),
+    (group, INVALID, [dict(ids=None), dict(adapters=0), dict(groups=None), dict(groups=P + 8)]),
     (group, TOO_LARGE, [dict(rows=1 << 28), dict(adapters=65536)]),
     (add, UNSUPPORTED, [dict(dt=F32), dict(dt=F8), dict(y_dt=I32)]),
-    (add, INVALID, [dict(y=None), dict(x=None), dict(A=None), dict(B=None), dict(groups=None), dict(groups=P + 4), dict(out=None), dict(ldy=31), dict(ldx=63), dict(ldo=31),
+    (add, INVALID, [dict(y=None), dict(x=None), dict(A=None), dict(B=None), dict(groups=None), dict(groups=P + 8), dict(out=None), dict(ldy=31), dict(ldx=63), dict(ldo=31),
                     dict(ldo=33), dict(adapters=0), dict(rank=0), dict(k=0), dict(n=0)]),
-    (add, TOO_LARGE, [dict(rows=1 << 28), dict(adapters=65536), dict(rank=129), dict(k=1 << 24), dict(n=1 << 24)]),
+    (add, TOO_LARGE, [dict(rows=1 << 28), dict(adapters=65536), dict(rank=129), dict(k=1 << 23), dict(n=1 << 23)]),
     (add_backward, UNSUPPORTED, [dict(dt=F32), dict(dx_dt=I8), dict(g_dt=I32)]),
-    (add_backward, INVALID, [dict(dy=None), dict(x=None), dict(u=None), dict(A=None), dict(B=None), dict(groups=None), dict(groups=P + 4), dict(dx=None), dict(lddy=31), dict(ldx=63),
+    (add_backward, INVALID, [dict(dy=None), dict(x=None), dict(u=None), dict(A=None), dict(B=None), dict(groups=None), dict(groups=P + 8), dict(dx=None), dict(lddy=31), dict(ldx=63),
                              dict(lddx=63), dict(lddx0=63), dict(dx=P, lddx=65), dict(adapters=0), dict(rank=0), dict(k=0), dict(n=0)]),
-    (add_backward, TOO_LARGE, [dict(rows=1 << 28), dict(adapters=65536), dict(rank=129), dict(k=1 << 24), dict(n=1 << 24)]),
+    (add_backward, TOO_LARGE, [dict(rows=1 << 28), dict(adapters=65536), dict(rank=129), dict(k=1 << 23), dict(n=1 << 23)]),
     (log_prob, UNSUPPORTED, [dict(dt=I8), dict(bytes=1)]),
     (log_prob, INVALID, [dict(x=None), dict(t=None), dict(logp=None), dict(entropy=None), dict(lse=None), dict(values=None), dict(indices=None), dict(ld=63), dict(cols=0), dict(top=-1),
                          dict(top=5, cols=4)]),
@@ -84,8 +84,8 @@ def test_nothing_to_do_needs_nothing():
 def test_words_of_groups():
     words = C.c_size_t()
     f = load_library().qgemm_group_rows_words
-    assert f(0, 1, C.byref(words)) == 0 and words.value == 6
-    assert f(1000, 7, C.byref(words)) == 0 and words.value == 1018 + 2 * (15 + 8)
+    assert f(0, 1, C.byref(words)) == 0 and words.value == 8
+    assert f(1000, 7, C.byref(words)) == 0 and words.value == 1020 + 4 * (15 + 8)
     assert f(4, 0, C.byref(words)) == INVALID and f(4, 1, None) == INVALID and f(4, 65536, C.byref(words)) == TOO_LARGE and f(1 << 28, 1, C.byref(words)) == TOO_LARGE
 
 
@@ -119,7 +119,7 @@ def check(what, status, most=128 << 20):
     for name, x, y, block in made:
         assert 0 < x * block < 1 << 32 and 0 < y < 1 << 16, (what, name, x, y, block)
     return took
-edges = [1, 7, 8, 64, 65, 16384, 16385, 1 << 18, 1 << 24, (1 << 24) - 256, 1 << 27, (1 << 28) - 1, 1 << 28, 1 << 30, (1 << 31) - 129, (1 << 31) - 128, (1 << 31) - 127, (1 << 31) - 1, 1 << 31]
+edges = [1, 7, 8, 64, 65, 16384, 16385, 1 << 18, 1 << 24, (1 << 23) - 256, 1 << 27, (1 << 28) - 1, 1 << 28, 1 << 30, (1 << 31) - 129, (1 << 31) - 128, (1 << 31) - 127, (1 << 31) - 1, 1 << 31]
 size = lambda most=31: rng.choice(edges) if rng.random() < 0.3 else int(2 ** rng.uniform(0, most))
 for _ in range(2000):
     rows, cols = size(), size()
