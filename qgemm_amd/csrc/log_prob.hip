@@ -17,7 +17,8 @@ auto with_type(int dt, F f) {
 }  // namespace
 
 size_t plan_log_prob(LogProbArgs &a, int cus) {
-    const uint32_t want = (uint32_t)cus * 4 / std::max<uint32_t>(a.rows, 1), most = (a.cols + kLogProbTurn - 1) / kLogProbTurn;
+    // (a part has one trip to memory's worth of columns for a workgroup: less gains nothing and leaves more to join)
+    const uint32_t trip = kLogProbAhead * kLogProbTurn, want = (uint32_t)cus * 4 / std::max<uint32_t>(a.rows, 1), most = (a.cols + trip - 1) / trip;
     a.splits = std::max<uint32_t>(1, std::min({want, most, kMostSplits}));
     a.part = ((a.cols + a.splits - 1) / a.splits + kOctet - 1) / kOctet * kOctet;
     a.splits = (a.cols + a.part - 1) / a.part;
@@ -30,7 +31,7 @@ hipError_t launch_log_prob(const LogProbArgs &a, hipStream_t stream) {
                              dim3(kLogProbThreads), 0, stream, a);
     });
     if (e != hipSuccess || a.splits == 1) return e;
-    return launch_kernel(log_prob_join_kernel, dim3(a.rows), dim3(64), 0, stream, a);
+    return launch_kernel(log_prob_join_kernel, dim3(a.rows), dim3(256), 0, stream, a);
 }
 
 hipError_t launch_log_prob_backward(const LogProbBackwardArgs &a, hipStream_t stream) {

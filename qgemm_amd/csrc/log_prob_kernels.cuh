@@ -94,20 +94,22 @@ __device__ __forceinline__ float logit_at(const void *row, int dt, size_t c) {
     const uint16_t h = ((const uint16_t *)row)[c];
     return dt == QGEMM_DT_BF16 ? __builtin_bit_cast(float, (uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
 }
-// a row's numbers out of its sums
-__device__ __forceinline__ float log_prob_finish(const LogProbArgs &p, uint32_t row, float m, float s, float t) {
-    const bool none = s == 0.0f;
-    const float l = logf(s), lse = none ? kMinusInf : m + l;
-    const int64_t token = token_at(p.tokens, p.token_bytes, row);
-    float lp = 0.0f;
-    if (token >= 0 && token < (int64_t)p.cols) {
-        const float x = logit_at((const char *)p.logits + (size_t)row * p.ld * dtype_bytes(p.dt), p.dt, (size_t)token);
-        lp = none ? kMinusInf : x - lse;
+// the logit that a row's token asks for, fetched ahead of its use: two trips to memory one behind the other
+struct Asked {
+    bool any;
+    float logit;
+    __device__ __forceinline__ Asked(const LogProbArgs &p, uint32_t row) {
+        const int64_t token = token_at(p.tokens, p.token_bytes, row);
+        any = token >= 0 && token < (int64_t)p.cols;
+        logit = logit_at((const char *)p.logits + (size_t)row * p.ld * dtype_bytes(p.dt), p.dt, any ? (size_t)token : 0);
     }
-    p.logp[row] = lp;
+};
+// a row's numbers out of its sums
+__device__ __forceinline__ void log_prob_finish(const LogProbArgs &p, uint32_t row, const Asked &asked, float s, float t, float l, float lse) {
+    const bool none = s == 0.0f;
+    p.logp[row] = !asked.any ? 0.0f : none ? kMinusInf : asked.logit - lse;
     p.entropy[row] = none ? 0.0f : l - t / s;
     p.lse[row] = lse;
-    return lse;
 }
 __device__ __forceinline__ void store_top(const LogProbArgs &p, uint32_t row, uint32_t place, uint64_t key, float lse) {
     const float v = value_of(key);
@@ -115,28 +117,44 @@ __device__ __forceinline__ void store_top(const LogProbArgs &p, uint32_t row, ui
     p.indices[(size_t)row * p.top + place] = index_of(key);
 }
 
-constexpr uint32_t kLogProbThreads = 256, kLogProbTurn = kLogProbThreads * kOctet, kCandidates = 2048;
+// how many of the first n keys of a list are above `mine`; the list has room for seven zeros behind them, and has them
+__device__ __forceinline__ uint32_t keys_above(const uint64_t *list, uint32_t n, uint64_t mine) {
+    uint32_t above = 0;
+    for (uint32_t k = 0; k < n; k += 8) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) above += list[k + i] > mine ? 1 : 0;
+    }
+    return above;
+}
+// the k-th largest of a wave's keys, of which no two are equal but zeros; 0 where there are fewer
+__device__ __forceinline__ uint64_t kth_largest(uint64_t mine, uint32_t k) {
+    uint32_t above = 0;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) above += key_lane(mine, i) > mine ? 1 : 0;
+    const uint64_t at = __ballot(above == k - 1 && mine != 0);
+    return at ? key_lane(mine, __builtin_ctzll(at)) : 0;
+}
+
+constexpr uint32_t kLogProbThreads = 256, kLogProbTurn = kLogProbThreads * kOctet, kLogProbAhead = 4, kCandidates = 2048;
 
 // The `top` largest of columns begin .. end - 1, `own` the key of a thread's largest octet (its value, its first column; 0: it has none), to
 // put(place, key) in place 0 .. top - 1, key 0 where there are fewer
 template <int DT, class Put>
 __device__ __forceinline__ void top_of(const void *row, uint32_t begin, uint32_t end, uint32_t top, uint64_t own, Put put) {
-    __shared__ uint64_t group[64], list[kCandidates];
+    __shared__ __align__(16) uint64_t group[64], list[kCandidates + 8];
     __shared__ uint32_t count, holders, holder[kLogProbThreads];
-    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const uint32_t tid = threadIdx.x;
     const uint64_t two = larger(own, key_dpp<0xB1>(own)), four = larger(two, key_dpp<0x4E>(two));
     if ((tid & 3) == 0) group[tid >> 2] = four;
     if (tid == 0) count = holders = 0;
     __syncthreads();
-    uint64_t least = 0;                                    // L
-    {
-        const uint64_t mine = group[lane];
-        uint32_t above = 0;
-#pragma unroll
-        for (int i = 0; i < 64; ++i) above += key_lane(mine, i) > mine ? 1 : 0;
-        const uint64_t at = __ballot(above == top - 1 && mine != 0);
-        if (at) least = key_lane(mine, __builtin_ctzll(at));
+    // (one wave for all: done by each of the four it was half of the time of rows of a thousand columns, 4096 x 1000 bf16 20 us)
+    if (tid < 64) {
+        const uint64_t least = kth_largest(group[tid], top);
+        if (tid == 0) list[0] = least;
     }
+    __syncthreads();
+    const uint64_t least = list[0];                        // L
     // an octet's key stands for any of its elements
     uint64_t bound = least == 0 ? 0 : (least & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (index_of(least) + kOctet - 1));
     if (own != 0 && own >= least) holder[atomicAdd(&holders, 1u)] = tid;
@@ -161,12 +179,12 @@ __device__ __forceinline__ void top_of(const void *row, uint32_t begin, uint32_t
         }
         __syncthreads();
         const uint32_t found = count, n = found < kCandidates ? found : kCandidates;
-        __syncthreads();                                   // (count is cleared below)
+        if (tid < 8) list[n + tid] = 0;
+        __syncthreads();                                   // (and count is cleared below)
         if (found <= kCandidates) {
             for (uint32_t i = tid; i < n; i += kLogProbThreads) {
                 const uint64_t mine = list[i];
-                uint32_t above = 0;
-                for (uint32_t k = 0; k < n; ++k) above += list[k] > mine ? 1 : 0;
+                const uint32_t above = keys_above(list, n, mine);
                 if (above < top) put(above, mine);
             }
             for (uint32_t i = n + tid; i < top; i += kLogProbThreads) put(i, 0ull);
@@ -176,9 +194,7 @@ __device__ __forceinline__ void top_of(const void *row, uint32_t begin, uint32_t
         // more than there is room for: the k-th largest of those that were kept is a higher bound still
         for (uint32_t i = tid; i < n; i += kLogProbThreads) {
             const uint64_t mine = list[i];
-            uint32_t above = 0;
-            for (uint32_t k = 0; k < n; ++k) above += list[k] > mine ? 1 : 0;
-            if (above == top - 1) group[0] = mine;
+            if (keys_above(list, n, mine) == top - 1) group[0] = mine;
         }
         if (tid == 0) count = 0;
         __syncthreads();
@@ -190,11 +206,12 @@ __device__ __forceinline__ void top_of(const void *row, uint32_t begin, uint32_t
 // one workgroup for a split of a row
 template <int DT, bool TOP>
 __global__ void __launch_bounds__(kLogProbThreads) log_prob_kernel(const LogProbArgs p) {
-    constexpr int AHEAD = 4, WAVES = kLogProbThreads / 64;
+    constexpr int AHEAD = kLogProbAhead, WAVES = kLogProbThreads / 64;
     __shared__ float red[3][WAVES];
     const uint32_t tid = threadIdx.x, begin = blockIdx.x * p.part, end = p.cols - begin < p.part ? p.cols : begin + p.part;
     for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
         const char *x = (const char *)p.logits + (size_t)row * p.ld * Octet<DT>::ES;
+        const Asked asked(p, row);
         Sums sums{kMinusInf, 0.0f, 0.0f};
         float best = kMinusInf;
         uint32_t best_at = begin + tid * kOctet;
@@ -239,6 +256,7 @@ __global__ void __launch_bounds__(kLogProbThreads) log_prob_kernel(const LogProb
             all_s += red[1][i];
             all_t += red[2][i];
         }
+        const float l = logf(all_s), lse = all_s == 0.0f ? kMinusInf : m + l;
         float *part = p.splits > 1 ? p.partial + ((size_t)row * p.splits + blockIdx.x) * log_prob_part(p.top) : nullptr;
         if (tid == 0) {
             if (part) {
@@ -246,12 +264,11 @@ __global__ void __launch_bounds__(kLogProbThreads) log_prob_kernel(const LogProb
                 part[1] = all_s;
                 part[2] = all_t;
             } else {
-                log_prob_finish(p, row, m, all_s, all_t);
+                log_prob_finish(p, row, asked, all_s, all_t, l, lse);
             }
         }
         if constexpr (TOP) {
             const uint64_t own = begin + tid * kOctet < end ? key_of(best, best_at) : 0;
-            const float lse = all_s == 0.0f ? kMinusInf : m + logf(all_s);
             top_of<DT>(x, begin, end, p.top, own, [&](uint32_t place, uint64_t key) {
                 if (part) ((uint64_t *)(part + 4))[place] = key;
                 else store_top(p, row, place, key, lse);
@@ -261,37 +278,54 @@ __global__ void __launch_bounds__(kLogProbThreads) log_prob_kernel(const LogProb
     }
 }
 
-// the splits of a row together, one wave a row: a lane has a split, and the largest of the splits' heads is the next of the top
-__global__ void __launch_bounds__(64) log_prob_join_kernel(const LogProbArgs p) {
-    __shared__ uint64_t heads[64 * kMostTop];
-    const uint32_t lane = threadIdx.x;
+// The splits of a row together.  Their lists are in order: where there are no fewer splits than places, the k-th largest of the heads is no more than the k-th
+// largest of all, else the smallest of what is in place k / splits, rounded up, of each; what reaches that is gathered and placed as above.
+__global__ void __launch_bounds__(256) log_prob_join_kernel(const LogProbArgs p) {
+    __shared__ __align__(16) uint64_t list[64 * kMostTop + 8];
+    __shared__ uint32_t count;
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
     for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const bool in = lane < p.splits;
-        const float *part = p.partial + ((size_t)row * p.splits + (in ? lane : 0)) * log_prob_part(p.top);
+        const Asked asked(p, row);
+        const float *parts = p.partial + (size_t)row * p.splits * log_prob_part(p.top), *part = parts + (in ? lane : 0) * log_prob_part(p.top);
+        constexpr uint32_t MOST = 64 * kMostTop / 256;
+        uint64_t own[MOST], bound = 0;
+        const uint32_t n = p.splits * p.top, place = p.top ? (p.top + p.splits - 1) / p.splits - 1 : 0;
+#pragma unroll
+        for (uint32_t i = 0; i < MOST; ++i) {
+            const uint32_t at = tid + i * 256;
+            own[i] = at < n ? ((const uint64_t *)(parts + at / p.top * log_prob_part(p.top) + 4))[at % p.top] : 0;
+        }
+        if (p.top) bound = ((const uint64_t *)(part + 4))[place];
         Sums sums{in ? part[0] : kMinusInf, in ? part[1] : 0.0f, in ? part[2] : 0.0f};
         const float m = wave_max(sums.m);
         sums.raise(m);
-        const float s = lanes_sum<64>(sums.s), t = lanes_sum<64>(sums.t), lse = s == 0.0f ? kMinusInf : m + logf(s);
-        if (lane == 0) log_prob_finish(p, row, m, s, t);
+        const float s = lanes_sum<64>(sums.s), t = lanes_sum<64>(sums.t), l = logf(s), lse = s == 0.0f ? kMinusInf : m + l;
+        if (tid == 0) log_prob_finish(p, row, asked, s, t, l, lse);
         if (!p.top) continue;
-        for (uint32_t i = lane; i < p.splits * p.top; i += 64)
-            heads[i] = ((const uint64_t *)(p.partial + ((size_t)row * p.splits + i / p.top) * log_prob_part(p.top) + 4))[i % p.top];
-        __syncthreads();
-        const uint64_t *own = heads + lane * p.top;
-        uint32_t next = 0;
-        uint64_t head = in ? own[0] : 0;
-        for (uint32_t i = 0; i < p.top; ++i) {
-            uint64_t most = head;
-            most = larger(most, key_dpp<0xB1>(most));
-            most = larger(most, key_dpp<0x4E>(most));
-            most = larger(most, key_dpp<0x141>(most));
-            most = larger(most, key_dpp<0x140>(most));
-            most = larger(larger(key_lane(most, 0), key_lane(most, 16)), larger(key_lane(most, 32), key_lane(most, 48)));
-            if (head == most && head != 0) {
-                store_top(p, row, i, most, lse);
-                ++next;
-                head = next < p.top ? own[next] : 0;
+        if (place == 0) {
+            bound = kth_largest(in ? bound : 0, p.top);
+        } else {
+            bound = in ? bound : ~0ull;
+#pragma unroll
+            for (int d = 32; d; d /= 2) {
+                const uint64_t other = __shfl_xor(bound, d);
+                bound = other < bound ? other : bound;
             }
+        }
+        if (tid == 0) count = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < MOST; ++i)
+            if (own[i] != 0 && own[i] >= bound) list[atomicAdd(&count, 1u)] = own[i];
+        __syncthreads();
+        const uint32_t found = count;
+        if (tid < 8) list[found + tid] = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < found; i += 256) {
+            const uint64_t mine = list[i];
+            const uint32_t above = keys_above(list, found, mine);
+            if (above < p.top) store_top(p, row, above, mine, lse);
         }
         __syncthreads();
     }
