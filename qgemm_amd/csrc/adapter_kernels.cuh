@@ -348,13 +348,14 @@ __global__ void __launch_bounds__(64 * kShrinkWaves, 4) adapter_shrink_kernel(co
 // and factor in flight behind a tile's products.  RANKS: the rank rounded up to 16, 32, 64 or 128;
 // ROW: see RowKind
 constexpr int kExpandCols = 128;
-template <int DT, int Y_DT, int RANKS>
+template <int DT, int Y_DT, int RANKS, int ROW>
 constexpr int expand_waves() {                                  // of a SIMD: what LDS and registers have room for
     const int lds = sum_parts<Y_DT>() * (int)kSlotRows * (RANKS * 2 + 16) + factor_parts<DT>() * 4 * Panel<2>::BYTES, fit = 160 * 1024 / lds;
-    return fit < 4 ? fit : 4;
+    const int most = Y_DT == QGEMM_DT_F32 && ROW == ROW_ANY ? 3 : 4;
+    return fit < most ? fit : most;
 }
 template <int DT, int Y_DT, int RANKS, int ROW>
-__global__ void __launch_bounds__(256, (expand_waves<DT, Y_DT, RANKS>())) adapter_expand_kernel(const ExpandArgs p) {
+__global__ void __launch_bounds__(256, (expand_waves<DT, Y_DT, RANKS, ROW>())) adapter_expand_kernel(const ExpandArgs p) {
     // PACKED (rank up to 16): two parts of u, 16 ranks each, make one product's 32
     constexpr bool PACKED = RANKS == 16;
     constexpr int PARTS = sum_parts<Y_DT>(), FACTORS = factor_parts<DT>(), STEP = PACKED ? 16 : 32, QUADS = RANKS / 4, PITCH = RANKS * 2 + 16;
@@ -368,15 +369,15 @@ __global__ void __launch_bounds__(256, (expand_waves<DT, Y_DT, RANKS>())) adapte
     const uint32_t ranks = plain ? 0 : p.rank, from = blockIdx.y * p.wide, to = p.cols - from < p.wide ? p.cols : from + p.wide;
     // (needs nothing but the slot)
     const uint32_t at_rank = lane >> 2, at_col = wave * 32 + (lane & 3) * 8;
-    Octet<DT> w[STEP / 16];
-    auto request_w = [&](uint32_t k, uint32_t tile) __attribute__((always_inline)) {
+    Octet<DT> w[RANKS / 16];                                     // of a whole tile: a wave has 16 ranks of 32 columns in one octet a lane
+    auto request_w = [&](uint32_t tile) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < STEP / 16; ++i) {
-            const uint32_t r = k + i * 16 + at_rank;
+        for (int i = 0; i < RANKS / 16; ++i) {
+            const uint32_t r = i * 16 + at_rank;
             w[i].template request<ROW>((const char *)p.w + ((size_t)s.adapter * p.rank + (r < p.rank ? r : p.rank - 1)) * p.cols * 2, tile + at_col, p.cols);
         }
     };
-    if (!plain) request_w(0, from);
+    if (!plain) request_w(from);
     Octet<Y_DT> y[4];
     uint32_t row[4];
 #pragma unroll
@@ -445,22 +446,24 @@ __global__ void __launch_bounds__(256, (expand_waves<DT, Y_DT, RANKS>())) adapte
         for (int f = 0; f < 4; ++f) {
             float v[8];
             y[f].template settle<ROW>(n, p.cols);
+            y[f].hold();
             y[f].floats(v);
             acc[f][0] = v4f{v[0], v[1], v[2], v[3]};
             acc[f][1] = v4f{v[4], v[5], v[6], v[7]};
         }
         if (then < to) request_y(then);
-#pragma unroll 1
-        for (uint32_t k = 0; k < ranks; k += STEP) {
+#pragma unroll
+        for (int k = 0; k < RANKS; k += STEP) {
+            if ((uint32_t)k >= ranks) break;
             // (a wave's panel is its own: what it writes and reads there comes in its own order)
 #pragma unroll
             for (int i = 0; i < STEP / 16; ++i) {
                 const uint32_t r = i * 16 + at_rank;
-                w[i].template settle<ROW>(k + r < p.rank ? tile + at_col : p.cols, p.cols);
-                stage_octet<DT, FACTORS>(w[i], panel + r * P::PITCH + (lane & 3) * 16, 4 * P::BYTES);
+                Octet<DT> &o = w[k / 16 + i];
+                o.template settle<ROW>(k + r < p.rank ? tile + at_col : p.cols, p.cols);
+                stage_octet<DT, FACTORS>(o, panel + r * P::PITCH + (lane & 3) * 16, 4 * P::BYTES);
             }
-            if (k + STEP < ranks) request_w(k + STEP, tile);
-            else if (then < to) request_w(0, then);
+            if ((uint32_t)k + STEP >= ranks && then < to) request_w(then);
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");

@@ -53,11 +53,11 @@ hipError_t launch_shrink(const ShrinkArgs &a, hipStream_t stream) {
     });
 }
 
-// Column tiles of a workgroup: as many as leave four workgroups a CU
+// Column tiles of a workgroup: as few as leave all workgroups room at the same time
 hipError_t launch_expand(ExpandArgs a, int cus, hipStream_t stream) {
-    const uint32_t tiles = (a.cols + kExpandCols - 1) / kExpandCols;
-    const uint64_t share = (uint64_t)a.g.slot_count * tiles / ((uint64_t)cus * 4), least = (tiles + 65534) / 65535;      // (launches of 2^16 workgroups down at the most)
-    const uint32_t each = (uint32_t)std::min<uint64_t>(tiles, std::max<uint64_t>({1, share, least}));
+    const uint32_t tiles = (a.cols + kExpandCols - 1) / kExpandCols, room = (uint32_t)cus * (a.rank <= 64 ? 4 : 3);
+    const uint32_t across = std::min<uint32_t>(std::max<uint32_t>(1, room / std::max<uint32_t>(a.g.slot_count, 1)), 65535);
+    const uint32_t each = (tiles + across - 1) / across;
     a.wide = each * kExpandCols;
     const dim3 grid(a.g.slot_count, (tiles + each - 1) / each);
     return with_dt(a.dt, [&](auto dt) {
