@@ -21,8 +21,22 @@ typedef __attribute__((address_space(3))) tr_v4s tr_quad;
 
 // ---- groups.  One workgroup for each group: how many rows come in front of it, in how many groups, then its rows in their order.  Slots: with o rows and
 // d groups in front, a group starts at slot o / 64 + d, and has room up to the next group's start, (o + n) / 64 + d + 1: at
-// least its n / 64 rounded up.  So every group finds its slots without knowing the others' sizes.
+// least its n / 64 rounded up.  So every group finds its slots without knowing the others' sizes.  Where there are more rows than adapters its number stands for d,
+// which is no smaller and needs no counting.
 //
+__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
+    auto dpp = [&](auto ctrl) { v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, true); };
+    dpp(std::integral_constant<int, 0xB1>{});
+    dpp(std::integral_constant<int, 0x4E>{});
+    dpp(std::integral_constant<int, 0x141>{});
+    dpp(std::integral_constant<int, 0x140>{});
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t a0 = a[0], a1 = a[1];
+    v = a0 + a1;
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const uint32_t b0 = b[0], b1 = b[1];
+    return b0 + b1;
+}
 // A thread has 4 neighbouring ids of each turn, of which TURNS stay in registers: of more rows all are read again for the second half.
 template <int ID_BYTES, int WAVES, int TURNS>
 __global__ void __launch_bounds__(64 * WAVES) group_rows_kernel(const void *ids, RowGroups g) {
@@ -52,48 +66,44 @@ __global__ void __launch_bounds__(64 * WAVES) group_rows_kernel(const void *ids,
         for (int e = 0; e < 4; ++e) of[e] = t + e >= g.rows ? 0xFFFFFFFFu : id[e] >= 0 && id[e] < (int64_t)none ? (uint32_t)id[e] : none;
     };
     static_assert(WAVES * TURNS <= 64, "a lane for each part of a turn");
-    for (uint32_t i = tid; i <= none / 32; i += THREADS) seen[i] = 0;
+    const bool marks = g.rows <= none;                      // groups in front of this one have to be counted
+    if (marks)
+        for (uint32_t i = tid; i <= none / 32; i += THREADS) seen[i] = 0;
     if (tid < 64) before[tid] = 0;
     uint32_t of[TURNS][4], less = 0, equal = 0;
 #pragma unroll
     for (uint32_t k = 0; k < TURNS; ++k) fetch(k * TURN + tid * 4, of[k]);
-    __syncthreads();
-    // (neighbours of one group, as prompts have them, mark it once)
+    if (marks) __syncthreads();
     auto count = [&](const uint32_t (&o)[4]) __attribute__((always_inline)) {
-        uint32_t last = __shfl_up(o[3], 1);
-        last = lane ? last : 0xFFFFFFFFu;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             equal += o[e] == a ? 1 : 0;
             less += o[e] < a ? 1 : 0;
-            if (o[e] < a && o[e] != last && !(seen[o[e] / 32] >> (o[e] % 32) & 1)) atomicOr(&seen[o[e] / 32], 1u << (o[e] % 32));
-            last = o[e];
+            if (marks && o[e] < a) atomicOr(&seen[o[e] / 32], 1u << (o[e] % 32));
         }
     };
 #pragma unroll
     for (uint32_t k = 0; k < TURNS; ++k) count(of[k]);
-    for (uint32_t t = TURNS * TURN; t < g.rows; t += TURN) {          // (all lanes of a wave together)
+    for (uint32_t t = TURNS * TURN + tid * 4; t < g.rows; t += TURN) {
         uint32_t o[4];
-        fetch(t + tid * 4, o);
+        fetch(t, o);
         count(o);
     }
-    __syncthreads();
     uint32_t distinct = 0;
-    for (uint32_t i = tid; i <= none / 32; i += THREADS) distinct += __builtin_popcount(seen[i]);
-    auto total = [&](uint32_t v) {
-#pragma unroll
-        for (int d = 32; d; d /= 2) v += __shfl_xor(v, d);
-        return v;
-    };
-    less = total(less), equal = total(equal), distinct = total(distinct);
+    if (marks) {
+        __syncthreads();
+        for (uint32_t i = tid; i <= none / 32; i += THREADS) distinct += __builtin_popcount(seen[i]);
+    }
+    less = wave_total(less), equal = wave_total(equal), distinct = wave_total(distinct);
     if (lane == 0) sums[wave][0] = less, sums[wave][1] = equal, sums[wave][2] = distinct;
     __syncthreads();
     less = equal = distinct = 0;
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) less += sums[i][0], equal += sums[i][1], distinct += sums[i][2];
+    if (!marks) distinct = a;
 
     const uint32_t slot = less / kSlotRows + distinct, filled = (equal + kSlotRows - 1) / kSlotRows;
-    const uint32_t behind = a == none ? g.slot_count : equal ? (less + equal) / kSlotRows + distinct + 1 : slot;
+    const uint32_t behind = a == none ? g.slot_count : !marks || equal ? (less + equal) / kSlotRows + distinct + 1 : slot;
     int32_t *order = const_cast<int32_t *>(g.order), *offsets = const_cast<int32_t *>(g.offsets), *first = const_cast<int32_t *>(g.first);
     v4i *slots = const_cast<v4i *>(g.slots);
     if (tid == 0) {
@@ -166,15 +176,18 @@ __device__ __forceinline__ uint16_t split_off(float &v) {
     v = __builtin_fabsf(rest) < __builtin_inff() ? rest : 0.0f;
     return h;
 }
-// four sums of a row from rank q on, those behind the last are 0; four parts of them in flight
+// the row of u that belongs to place `at` of the order
+__device__ __forceinline__ uint32_t sums_row(const RankSums &u, const RowGroups &g, uint32_t at) { return u.grouped ? at : (uint32_t)g.order[at]; }
+// four sums of a row from rank q on, those behind the last are 0; four or eight parts of them in flight
 __device__ __forceinline__ v4f rank_sums(const RankSums &u, size_t row, uint32_t q, uint32_t rank) {
     v4f sum = {};
     const float *at = u.at + row * u.pitch + q;
     if (u.planes == 1 && q + 4 <= rank) return *(const v4f_any *)at;
-    for (uint32_t i = 0; i < u.planes; i += 4) {
-        v4f part[4];
+    auto add = [&](auto flight, uint32_t i) __attribute__((always_inline)) {
+        constexpr uint32_t N = decltype(flight)::value;
+        v4f part[N];
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
+        for (uint32_t k = 0; k < N; ++k) {
             const float *p = at + (i + k < u.planes ? i + k : i) * u.stride;
             if (q + 4 <= rank) {
                 part[k] = *(const v4f_any *)p;
@@ -183,11 +196,13 @@ __device__ __forceinline__ v4f rank_sums(const RankSums &u, size_t row, uint32_t
                 for (uint32_t e = 0; e < 4; ++e) part[k][e] = q + e < rank ? p[e] : 0.0f;
             }
         }
-        sum += part[0];
 #pragma unroll
-        for (uint32_t k = 1; k < 4; ++k)
+        for (uint32_t k = 0; k < N; ++k)
             if (i + k < u.planes) sum += part[k];
-    }
+    };
+    if (u.planes <= 4) add(std::integral_constant<uint32_t, 4>{}, 0);
+    else
+        for (uint32_t i = 0; i < u.planes; i += 8) add(std::integral_constant<uint32_t, 8>{}, i);
     return sum;
 }
 // A panel is up to 32 rows of 16 FC columns of 16 bits, a wave's own.  `columns` gives the matrix cores' operand along the rows: lane j of a group of 16 supplies
@@ -251,7 +266,7 @@ __global__ void __launch_bounds__(64 * kShrinkWaves, 4) adapter_shrink_kernel(co
         const uint32_t wide = p.u.pitch < RANKS ? p.u.pitch : RANKS;
         for (uint32_t i = tid; i < s.count * RANKS; i += THREADS) {
             const uint32_t row = i / RANKS, k = i % RANKS;
-            if (k < wide) u[(size_t)(uint32_t)p.g.order[s.begin + row] * p.u.pitch + k] = k < p.rank ? value(row, k) : 0.0f;
+            if (k < wide) u[(size_t)sums_row(p.u, p.g, s.begin + row) * p.u.pitch + k] = k < p.rank ? value(row, k) : 0.0f;
         }
     };
     if (s.adapter == p.g.adapters) {
@@ -351,7 +366,8 @@ constexpr int kExpandCols = 128;
 template <int DT, int Y_DT, int RANKS, int ROW>
 constexpr int expand_waves() {                                  // of a SIMD: what LDS and registers have room for
     const int lds = sum_parts<Y_DT>() * (int)kSlotRows * (RANKS * 2 + 16) + factor_parts<DT>() * 4 * Panel<2>::BYTES, fit = 160 * 1024 / lds;
-    const int most = Y_DT == QGEMM_DT_F32 && ROW == ROW_ANY ? 3 : 4;
+    constexpr bool more = Y_DT == QGEMM_DT_F16 || ROW == ROW_ANY;
+    const int most = RANKS < 64 ? (more ? 3 : 4) : more ? 2 : Y_DT == QGEMM_DT_F32 ? 3 : 4;
     return fit < most ? fit : most;
 }
 template <int DT, int Y_DT, int RANKS, int ROW>
@@ -396,12 +412,12 @@ __global__ void __launch_bounds__(256, (expand_waves<DT, Y_DT, RANKS, ROW>())) a
     request_y(from);
     const float by = plain || !p.scaling ? 1.0f : p.scaling[s.adapter];
     // the rank's sums of the slot's rows, in parts: a lane has EACH quads of them (what lies behind the rows goes into products that nobody stores)
-    constexpr int EACH = (int)kSlotRows * QUADS / 256, BATCH = EACH < 2 ? 1 : 2;
+    constexpr int EACH = (int)kSlotRows * QUADS / 256, BATCH = 1;
     uint32_t sum_row[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         const uint32_t at = (tid + 256 * i) / QUADS;
-        sum_row[i] = (uint32_t)p.g.order[s.begin + (at < s.count ? at : s.count - 1)];
+        sum_row[i] = sums_row(p.u, p.g, s.begin + (at < s.count ? at : s.count - 1));
     }
 #pragma unroll
     for (int i0 = 0; i0 < EACH; i0 += BATCH) {
@@ -416,10 +432,12 @@ __global__ void __launch_bounds__(256, (expand_waves<DT, Y_DT, RANKS, ROW>())) a
             const uint32_t n = tid + 256 * (i0 + i), at = n / QUADS, q = n % QUADS * 4;
             if (at >= s.count) break;
             v4f v = sum[i];
-            if (p.keep && blockIdx.y == 0)
+            if (p.keep && blockIdx.y == 0) {
+                const size_t to_row = p.keep_grouped ? s.begin + at : (uint32_t)p.g.order[s.begin + at];
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e)
-                    if (q + e < p.rank) p.keep[(size_t)sum_row[i0 + i] * p.rank + q + e] = v[e];
+                    if (q + e < p.rank) p.keep[to_row * p.rank + q + e] = v[e];
+            }
             v *= by;
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) {
@@ -554,11 +572,11 @@ __global__ void __launch_bounds__(RT == 8 ? 512 : 256) adapter_grad_kernel(const
     };
     const uint32_t c = c0 + (lane & 7) * 8, octet0 = (wave >> 2) * OCTETS;      // a lane's octets: rows 8 (octet0 + i) + lane / 8 of the step
     auto rows_of = [&](Rows &r, uint32_t t) __attribute__((always_inline)) {
-        auto at = [&](uint32_t i) { return (uint32_t)p.g.order[i < to ? i : to - 1]; };
+        auto at = [&](uint32_t i) { return i < to ? i : to - 1; };
 #pragma unroll
-        for (int i = 0; i < OCTETS; ++i) r.z[i] = at(t + (octet0 + i) * 8 + (lane >> 3));
+        for (int i = 0; i < OCTETS; ++i) r.z[i] = (uint32_t)p.g.order[at(t + (octet0 + i) * 8 + (lane >> 3))];
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) r.u[i] = at(t + (tid + THREADS * i) / (RANKS / 4) % 32);
+        for (int i = 0; i < LOADS; ++i) r.u[i] = sums_row(of.u, p.g, at(t + (tid + THREADS * i) / (RANKS / 4) % 32));
     };
     auto request = [&](Step &b, const Rows &r) __attribute__((always_inline)) {
 #pragma unroll

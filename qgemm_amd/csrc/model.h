@@ -78,6 +78,7 @@ struct RankSums {
     float *at;
     uint64_t stride;                     // from a part to the next
     uint32_t pitch, planes;              // pitch: from a row to the next
+    int grouped;                         // the rows lie as they are grouped, so that nothing has to be looked up for them
 };
 inline uint32_t rank_pitch(uint32_t rank) { return (rank + 15) / 16 * 16; }
 
@@ -98,6 +99,7 @@ struct ExpandArgs {                      // out[row] = y[row] + scaling[its adap
     const float *scaling;                // null: 1
     void *out;
     float *keep;                         // u's parts added up, [rows][rank], or null
+    int keep_grouped;
     RankSums u;
     uint64_t ldy, ldo;
     uint32_t cols, rank, wide;           // wide: columns of a workgroup

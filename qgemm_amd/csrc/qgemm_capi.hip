@@ -1853,6 +1853,7 @@ size_t plan_rank_sums(ShrinkArgs &s, float *u) {
         return 0;
     }
     s.u.pitch = rank_pitch(s.rank);
+    s.u.grouped = 1;
     s.u.stride = (uint64_t)s.g.rows * s.u.pitch;
     return s.u.planes * s.u.stride * sizeof(float);
 }
@@ -2379,7 +2380,7 @@ QGEMM_EXPORT int qgemm_add_adapters_backward(int dtype, int dx_dtype, int grad_d
     g.dt = dtype, g.dw_dt = grad_dtype;
     g.of[0].z = x, g.of[0].dw = dA, g.of[0].ldz = ldx, g.of[0].cols = (uint32_t)k, g.of[0].u = s.u;
     g.of[1].z = dy, g.of[1].dw = dB, g.of[1].ldz = lddy, g.of[1].cols = (uint32_t)n;
-    g.of[1].u = RankSums{const_cast<float *>(u), 0, (uint32_t)rank, 1};
+    g.of[1].u = RankSums{const_cast<float *>(u), 0, (uint32_t)rank, 1, 0};
     const size_t room = dA || dB ? plan_adapter_grad(g, g_ctx.num_cus) : 0;
     void *ws = nullptr;
     if (sums + joined + room) {
@@ -2387,7 +2388,7 @@ QGEMM_EXPORT int qgemm_add_adapters_backward(int dtype, int dx_dtype, int grad_d
         if (st != QGEMM_OK) return st;
         s.u.at = (float *)ws;
         float *v = (float *)((char *)ws + sums);
-        g.of[0].u = joined ? RankSums{v, 0, (uint32_t)rank, 1} : s.u;
+        g.of[0].u = joined ? RankSums{v, 0, (uint32_t)rank, 1, 1} : s.u;
         place_adapter_grad(g, (float *)((char *)ws + sums + joined));
     }
     g_ctx.last_config = "add_adapters_backward";
@@ -2395,6 +2396,7 @@ QGEMM_EXPORT int qgemm_add_adapters_backward(int dtype, int dx_dtype, int grad_d
     if (rows && dx) {
         ExpandArgs e = expand_args(s, dx_dtype, A, scaling, dx0, dx0 ? lddx0 : lddx, dx, lddx, k);
         e.keep = joined ? (float *)((char *)ws + sums) : nullptr;
+        e.keep_grouped = 1;
         if (launch_expand(e, g_ctx.num_cus, stream) != hipSuccess) return QGEMM_ERR_LAUNCH;
     }
     if (!dA && !dB) return QGEMM_OK;
