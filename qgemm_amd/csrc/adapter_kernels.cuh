@@ -10,6 +10,11 @@
 // u and v are fp32.  Where they are an operand of the matrix cores they are split into bf16 numbers that add up to them, two of them (16 bits) where
 // the result has 16 bits, three (24) where it has 32; fp16 operands beside them are split into two, exactly, which keeps bf16's exponents:
 // gradients are often below what fp16 holds.
+//
+// What bounds them, times of the kernels in a trace: memory, and for few rows the chain of trips to it (slot, order, operands) behind a launch.  64 rows of 48 adapters of
+// rank 16, 4096 x 4096: group 2.8 us, shrink 4.4, expand 6.4; 8192 rows of 8 adapters of rank 32: 6.2, 16.6 and 31.2 (4.0 TB/s of x; 4.3 of y in and out).  Backward of 4096 rows of
+// 16 adapters of rank 16, 2048 x 8192: 5.7, 19.2, 12.5, both gradients 23.6 and their parts' sums 6.5.  High ranks read the factors out of the L2 once
+// a slot: shrink of 8192 rows of 8192 at rank 16 26.7 and at rank 64 50, 2048 rows at rank 128 46.
 #pragma once
 #include "model.h"
 #include "octet.cuh"
@@ -22,7 +27,7 @@ typedef __attribute__((address_space(3))) tr_v4s tr_quad;
 // ---- groups.  One workgroup for each group: how many rows come in front of it, in how many groups, then its rows in their order.  Slots: with o rows and
 // d groups in front, a group starts at slot o / 64 + d, and has room up to the next group's start, (o + n) / 64 + d + 1: at
 // least its n / 64 rounded up.  So every group finds its slots without knowing the others' sizes.  Where there are more rows than adapters its number stands for d,
-// which is no smaller and needs no counting.
+// which is no smaller and needs no counting (8192 rows 7.8 us with it, 6.2 without).
 //
 __device__ __forceinline__ uint32_t wave_total(uint32_t v) {
     auto dpp = [&](auto ctrl) { v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, true); };
@@ -246,7 +251,8 @@ constexpr int sum_parts() { return Y_DT == QGEMM_DT_F32 ? 3 : 2; }
 
 // ---- shrink: both operands straight from memory to the matrix cores' registers; a lane takes 16 neighbouring columns of a row for two products, and four lanes a
 // whole line.  The waves of a workgroup share its split's columns out between them, and ranks beyond 32 between two or four of them, which read the same rows.  Their sums meet in
-// LDS, in BUFFERS places one after the other.
+// LDS, in BUFFERS places one after the other.  (8192 x 4096 at rank 32: four waves of 256 columns by three splits 23.5 us, half lines a request with a step ahead in flight
+// 23.2, whole lines 21.2, and 16.6 with a fourth split, so that every CU has its two workgroups.  Sixteen waves a workgroup, one a CU: 27.)
 constexpr int kShrinkWaves = 8;
 template <int RT>
 struct ShrinkShape {
@@ -362,6 +368,8 @@ __global__ void __launch_bounds__(64 * kShrinkWaves, 4) adapter_shrink_kernel(co
 // ---- expand: 32 columns a wave, all rows of the slot; y is what the accumulators start with.  A workgroup goes over `wide` columns, 128 at a time, the next tile's y
 // and factor in flight behind a tile's products.  RANKS: the rank rounded up to 16, 32, 64 or 128;
 // ROW: see RowKind
+// (8192 x 4096 at rank 32: one tile of 256 columns a workgroup, everything loaded where it is wanted, 45 us; loads in front 37; 128 columns, several tiles a workgroup, 33;
+// the factor of a whole tile a tile ahead, no more workgroups than run at a time 31.  Eight waves a workgroup: 32.  Rank 128, 2048 x 8192: 91, 49 and 35.)
 constexpr int kExpandCols = 128;
 template <int DT, int Y_DT, int RANKS, int ROW>
 constexpr int expand_waves() {                                  // of a SIMD: what LDS and registers have room for
@@ -531,7 +539,9 @@ __host__ __device__ inline uint32_t adapter_plane_cols(uint32_t cols) { return (
 
 //
 // Both factors' gradients are one launch: x counts slots, and behind them adapters, for those that have no rows; y the column tiles of the first and then of the
-// second.  A step's loads are requested a step ahead, the numbers of its rows two.
+// second.  A step's loads are requested a step ahead, the numbers of its rows two.  (Both factors of 4096 rows, 2048 x 8192 at rank 16: two launches without loads ahead 65 us
+// and 10 for their parts; 23.6 and 6.5.  u and v lie in LDS as rows, as they come, and are turned by the transposing reads: written turned, by elements, 2048 rows
+// of 8192 at rank 128 took 150, 76 so.)
 template <int DT, int RT, int PARTS>
 struct GradRoom {
     static constexpr int BYTES = 2 * (PARTS * 32 * (RT * 32 + 16) + factor_parts<DT>() * 4 * Panel<4>::BYTES);

@@ -11,6 +11,10 @@
 // reaches L hold any element that does.  Their columns are read once more, what reaches L is gathered, and an element's place is the
 // number of those above it.  Elements are compared as 64-bit keys, value above, then the lower index: no two are equal, and the order is that of
 // the values with ties to the lowest index.
+//
+// What bounds it: memory, with the vector instructions (eleven slots an element, four of them the exponential) close behind: 2048 x 65536 bf16 with five tokens 61 us in a
+// trace, 4.4 TB/s; a plain sum of as many bytes reads 4.0.  8 x 131072 fp32 with twenty tokens 7.3 and 5 for the join, trips to memory and to LDS one behind
+// the other; backward 2048 x 65536 bf16 116, 4.6 TB/s read and written.
 #pragma once
 #include "model.h"
 #include "octet.cuh"
@@ -279,7 +283,8 @@ __global__ void __launch_bounds__(kLogProbThreads) log_prob_kernel(const LogProb
 }
 
 // The splits of a row together.  Their lists are in order: where there are no fewer splits than places, the k-th largest of the heads is no more than the k-th
-// largest of all, else the smallest of what is in place k / splits, rounded up, of each; what reaches that is gathered and placed as above.
+// largest of all, else the smallest of what is in place k / splits, rounded up, of each; what reaches that is gathered and placed as above.  (One wave that takes the largest
+// head k times: 13 us for 64 splits with twenty tokens; 5.)
 __global__ void __launch_bounds__(256) log_prob_join_kernel(const LogProbArgs p) {
     __shared__ __align__(16) uint64_t list[64 * kMostTop + 8];
     __shared__ uint32_t count;
