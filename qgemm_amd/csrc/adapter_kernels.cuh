@@ -429,6 +429,7 @@ __global__ void __launch_bounds__(256, (expand_waves<DT, Y_DT, RANKS, ROW>())) a
     }
 #pragma unroll
     for (int i0 = 0; i0 < EACH; i0 += BATCH) {
+        if (256 * i0 / QUADS >= (int)s.count) break;
         v4f sum[BATCH];
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
