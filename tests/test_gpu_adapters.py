@@ -72,7 +72,8 @@ def check_backward(dy, x, u, A, B, ids, scaling, dx, grad_dtype=F32):
 
 
 @pytest.mark.parametrize("rows,adapters,kind", [(1, 1, "one"), (1, 3, "none"), (5, 40, "mixed"), (64, 48, "mixed"), (200, 3, "runs"), (1000, 7, "mixed"), (129, 2, "none"),
-                                                (4097, 300, "mixed"), (3000, 1, "one"), (70, 65535, "mixed"), (0, 5, "mixed")])
+                                                (4097, 300, "mixed"), (3000, 1, "one"), (70, 65535, "mixed"), (0, 5, "mixed"), (16384, 3, "runs"), (16385, 5, "mixed"), (40001, 7, "mixed"), (40000, 2, "runs"), (20000, 30000, "mixed"),
+                                                (257, 257, "mixed"), (256, 256, "runs"), (2049, 2048, "mixed"), (2048, 2049, "mixed")])
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
 def test_groups(rows, adapters, kind, dtype):
     """Rows group by group in their own order, and slots that cover every group in pieces of up to 64."""
@@ -129,6 +130,17 @@ def test_gradients_of_many_rows():
     _, dA, dB = check_backward(values((rows, n), BF16, 6, n ** -0.5), x, u, A, B, ids, s, None)
     for i in (1, 3, 5, 6, 8):
         assert (dA[i] == 0).all() and (dB[i] == 0).all()
+
+
+@pytest.mark.parametrize("rows", [17000, 40000])
+def test_many_rows(rows):
+    """More rows than a group's registers hold ids of, forward against 64 bits, and gradients of sums in many parts."""
+    say("add_adapters many rows", rows)
+    adapters, rank, k, n = 5, 8, 64, 72
+    y, x, A, B, s = operands(rows, adapters, rank, k, n, BF16, BF16, 50)
+    ids = ids_of(rows, adapters, "mixed", 51)
+    _, u, _ = check(y, x, A, B, ids, s)
+    check_backward(values((rows, n), BF16, 52, n ** -0.5), x, u, A, B, ids, s, None)
 
 
 def test_small_gradients_of_fp16():

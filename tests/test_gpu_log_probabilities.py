@@ -85,6 +85,20 @@ def test_ties_go_to_the_lowest_token(cols, dtype):
     check(x, tokens_of(7, cols, 3), min(32, cols))
 
 
+@pytest.mark.parametrize("rows,cols", [(3, 40000), (1100, 20000)])
+@pytest.mark.parametrize("groups", [31, 8, 1])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_more_candidates_than_there_is_room_for(rows, cols, groups, dtype):
+    """All that is large lies in the columns of a few threads, so that the first bound lets thousands of elements through; in rising order every one is above those before."""
+    say("log_probabilities candidates", rows, cols, groups, dtype)
+    x = logits_of(rows, cols, dtype, 4) - 20
+    own = torch.arange(cols, device="cuda") // 8 % 256 < 4 * groups
+    x[:, own] += 20
+    x[1, own] = torch.arange(int(own.sum()), device="cuda").to(dtype) / 1024
+    x[2, own] = 3.0
+    check(x, tokens_of(rows, cols, 5), 32)
+
+
 @pytest.mark.parametrize("cols", [40, 3000, 70001])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_masks(cols, dtype):
