@@ -35,7 +35,8 @@ hipError_t launch_log_prob(const LogProbArgs &a, hipStream_t stream) {
 }
 
 hipError_t launch_log_prob_backward(const LogProbBackwardArgs &a, hipStream_t stream) {
-    const uint32_t across = std::min<uint32_t>((a.cols + kLogProbTurn - 1) / kLogProbTurn, 64);
+    // (two octets of a thread: us, 2048 x 65536 bf16 with one / two / four 115 / 92 / 93)
+    const uint32_t across = std::min<uint32_t>((a.cols + 2 * kLogProbTurn - 1) / (2 * kLogProbTurn), 64);
     return with_type(a.dt, [&](auto dt) {
         return launch_kernel(log_prob_backward_kernel<dt.value>, dim3(across, std::min(a.rows, kMostRowGroups)), dim3(kLogProbThreads), 0, stream, a);
     });

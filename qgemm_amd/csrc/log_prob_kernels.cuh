@@ -14,7 +14,7 @@
 //
 // What bounds it: memory, with the vector instructions (eleven slots an element, four of them the exponential) close behind: 2048 x 65536 bf16 with five tokens 61 us in a
 // trace, 4.4 TB/s; a plain sum of as many bytes reads 4.0.  8 x 131072 fp32 with twenty tokens 7.3 and 5 for the join, trips to memory and to LDS one behind
-// the other; backward 2048 x 65536 bf16 116, 4.6 TB/s read and written.
+// the other; backward 2048 x 65536 bf16 92, 5.9 TB/s read and written.
 #pragma once
 #include "model.h"
 #include "octet.cuh"
@@ -336,9 +336,10 @@ __global__ void __launch_bounds__(256) log_prob_join_kernel(const LogProbArgs p)
     }
 }
 
-// ---- backward: a workgroup takes kLogProbTurn columns a turn
+// ---- backward: a workgroup takes AHEAD times kLogProbTurn columns a turn
 template <int DT>
 __global__ void __launch_bounds__(kLogProbThreads) log_prob_backward_kernel(const LogProbBackwardArgs p) {
+    constexpr uint32_t AHEAD = 2;
     for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
         const char *x = (const char *)p.logits + (size_t)row * p.ld * Octet<DT>::ES;
         char *dx = (char *)p.dlogits + (size_t)row * p.ldd * dtype_bytes(p.out_dt);
@@ -347,23 +348,29 @@ __global__ void __launch_bounds__(kLogProbThreads) log_prob_backward_kernel(cons
         const float lse = p.lse[row], b = p.dentropy ? p.dentropy[row] : 0.0f, h = b != 0.0f ? p.entropy[row] : 0.0f;
         const bool none = lse == kMinusInf;
         const float a = asked && !none ? p.dlogp[row] : 0.0f;
-        for (uint32_t c = (blockIdx.x * kLogProbThreads + threadIdx.x) * kOctet; c < p.cols; c += gridDim.x * kLogProbTurn) {
-            Octet<DT> o;
-            float v[8];
-            o.request(x, c, p.cols);
-            o.settle(c, p.cols);
-            o.floats(v);
+        for (uint32_t c0 = blockIdx.x * AHEAD * kLogProbTurn + threadIdx.x * kOctet; c0 < p.cols; c0 += gridDim.x * AHEAD * kLogProbTurn) {
+            Octet<DT> o[AHEAD];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float l = v[e] - lse, q = none ? 0.0f : exp_of(l);
-                const float g = a + b * (__builtin_fmaxf(l, kNothing) + h);
-                v[e] = -(q * g);
-                if (asked && (int64_t)(c + e) == token) v[e] += a;
+            for (int i = 0; i < AHEAD; ++i) o[i].request(x, c0 + i * kLogProbTurn, p.cols);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const uint32_t c = c0 + i * kLogProbTurn;
+                if (c >= p.cols) break;
+                float v[8];
+                o[i].settle(c, p.cols);
+                o[i].floats(v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float l = v[e] - lse, q = none ? 0.0f : exp_of(l);
+                    const float g = a + b * (__builtin_fmaxf(l, kNothing) + h);
+                    v[e] = -(q * g);
+                    if (asked && (int64_t)(c + e) == token) v[e] += a;
+                }
+                if (none)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+                store_octet(dx, p.out_dt, c, p.cols, v);
             }
-            if (none)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-            store_octet(dx, p.out_dt, c, p.cols, v);
         }
     }
 }
