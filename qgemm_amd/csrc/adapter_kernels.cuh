@@ -678,31 +678,33 @@ __global__ void __launch_bounds__(RT == 8 ? 512 : 256) adapter_grad_kernel(const
     }
 }
 
-// groups of several parts, added up in their order: a workgroup has up to 2048 columns of one rank of one adapter
+// groups of several parts, added up in their order: a workgroup has 2048 columns at a time of every p.join-th rank of one adapter
 __global__ void __launch_bounds__(256) adapter_grad_join_kernel(const AdapterGradArgs p) {
     const AdapterGrad &of = p.of[blockIdx.z];
-    const uint32_t a = blockIdx.x / p.rank, k = blockIdx.x % p.rank, rows = (uint32_t)p.g.offsets[a + 1] - (uint32_t)p.g.offsets[a];
-    const uint32_t slots = (rows + kSlotRows - 1) / kSlotRows;
-    if (slots <= p.chunk || !of.dw) return;
+    const uint32_t a = blockIdx.x / p.join, rows = (uint32_t)p.g.offsets[a + 1] - (uint32_t)p.g.offsets[a], slots = (rows + kSlotRows - 1) / kSlotRows;
     const uint32_t wide = adapter_plane_cols(of.cols), first = (uint32_t)p.g.first[a];
-    char *out = (char *)of.dw + ((size_t)a * p.rank + k) * of.cols * dtype_bytes(p.dw_dt);
-    for (uint32_t c = (blockIdx.y * 256 + threadIdx.x) * kOctet; c < of.cols; c += gridDim.y * 2048) {
-        v4f lo = {}, hi = {};
-        for (uint32_t at = 0; at < slots; at += p.chunk * 4) {
-            v4f part[4][2];
+    if (slots <= p.chunk || !of.dw) return;
+#pragma unroll 1
+    for (uint32_t k = blockIdx.x % p.join; k < p.rank; k += p.join) {
+        char *out = (char *)of.dw + ((size_t)a * p.rank + k) * of.cols * dtype_bytes(p.dw_dt);
+        for (uint32_t c = (blockIdx.y * 256 + threadIdx.x) * kOctet; c < of.cols; c += gridDim.y * 2048) {
+            v4f lo = {}, hi = {};
+            for (uint32_t at = 0; at < slots; at += p.chunk * 4) {
+                v4f part[4][2];
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t j = at + i * p.chunk < slots ? at + i * p.chunk : at;
-                const float *plane = of.room + (grad_plane_of(first + j, p.chunk, j > 0) * p.rank + k) * wide + c;
-                part[i][0] = *(const v4f *)plane;
-                part[i][1] = *(const v4f *)(plane + 4);
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t j = at + i * p.chunk < slots ? at + i * p.chunk : at;
+                    const float *plane = of.room + (grad_plane_of(first + j, p.chunk, j > 0) * p.rank + k) * wide + c;
+                    part[i][0] = *(const v4f *)plane;
+                    part[i][1] = *(const v4f *)(plane + 4);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+                    if (at + i * p.chunk < slots) lo += part[i][0], hi += part[i][1];
             }
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-                if (at + i * p.chunk < slots) lo += part[i][0], hi += part[i][1];
+            const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            store_octet(out, p.dw_dt, c, of.cols, v);
         }
-        const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        store_octet(out, p.dw_dt, c, of.cols, v);
     }
 }
 

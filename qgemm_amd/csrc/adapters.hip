@@ -19,6 +19,13 @@ auto with_ranks(uint32_t rank, F f) {
     if (rank <= 64) return f(std::integral_constant<int, 4>{});
     return f(std::integral_constant<int, 8>{});
 }
+// Slots that there are likely to be, by which work is shared out: of a few rows any may have an adapter of its own, many are prompts, and of the adapters
+// that there is room for most have no row.  (8192 rows of 32 prompts, 4096 x 4096 at rank 16, 1000 adapters, us: shrink and expand by the slots that there could be
+// 45 and 138, by these 27 and 75.)
+uint32_t likely_slots(const RowGroups &g) {
+    const uint32_t whole = g.rows / kSlotRows;
+    return std::max<uint32_t>(1, std::min(g.slot_count, whole + std::min(g.adapters + 1, std::max<uint32_t>(64, whole))));
+}
 uint32_t column_tiles(uint32_t cols) { return (cols + 255) / 256; }
 }  // namespace
 
@@ -35,7 +42,7 @@ hipError_t launch_group_rows(const void *ids, int id_bytes, const RowGroups &g, 
 // Splits of the columns until the CUs' two workgroups each are all there, each wave on 64 columns or more (us, 8192 rows x 8192 in 137 slots, rank 16, 1 / 2 / 3 / 4 / 6 / 8 /
 // 16 splits: 39 / 41 / 33 / 27 / 30 / 28 / 30 on the same buffers again, 71 / 73 / 59 / 45 / 57 / 52 / 54 out of HBM)
 void plan_shrink(ShrinkArgs &a, int cus) {
-    const uint32_t least = kShrinkWaves * 64, most = (a.cols + least - 1) / least, slots = std::max<uint32_t>(a.g.slot_count, 1);
+    const uint32_t least = kShrinkWaves * 64, most = (a.cols + least - 1) / least, slots = likely_slots(a.g);
     const uint32_t splits = std::min({((uint32_t)cus * 2 + slots - 1) / slots, most, 16u});
     a.part = ((a.cols + splits - 1) / splits + least - 1) / least * least;
     a.u.planes = (a.cols + a.part - 1) / a.part;
@@ -56,7 +63,7 @@ hipError_t launch_shrink(const ShrinkArgs &a, hipStream_t stream) {
 // Column tiles of a workgroup: as few as leave all workgroups room at the same time
 hipError_t launch_expand(ExpandArgs a, int cus, hipStream_t stream) {
     const uint32_t tiles = (a.cols + kExpandCols - 1) / kExpandCols, room = (uint32_t)cus * (a.rank <= 64 ? 4 : 3);
-    const uint32_t across = std::min<uint32_t>(std::max<uint32_t>(1, room / std::max<uint32_t>(a.g.slot_count, 1)), 65535);
+    const uint32_t across = std::min<uint32_t>(std::max<uint32_t>(1, room / likely_slots(a.g)), 65535);
     const uint32_t each = (tiles + across - 1) / across;
     a.wide = each * kExpandCols;
     const dim3 grid(a.g.slot_count, (tiles + each - 1) / each);
@@ -93,7 +100,7 @@ void place_adapter_grad(AdapterGradArgs &a, float *room) {
     a.of[1].room = (float *)((char *)room + grad_room(a, 0));
 }
 
-hipError_t launch_adapter_grad(const AdapterGradArgs &a, hipStream_t stream) {
+hipError_t launch_adapter_grad(AdapterGradArgs a, hipStream_t stream) {
     const dim3 grid(a.g.slot_count + a.g.adapters, a.tiles + column_tiles(a.of[1].cols));
     const hipError_t e = with_dt(a.dt, [&](auto dt) {
         return with_ranks(a.rank, [&](auto rt) {
@@ -111,8 +118,10 @@ hipError_t launch_adapter_grad(const AdapterGradArgs &a, hipStream_t stream) {
         });
     });
     if (e != hipSuccess || grad_room(a, 0) + grad_room(a, 1) == 0) return e;
-    const uint32_t across = (std::max(a.of[0].cols, a.of[1].cols) + 2047) / 2048;
-    return launch_kernel(adapter_grad_join_kernel, dim3(a.g.adapters * a.rank, std::min<uint32_t>(across, 64), 2), dim3(256), 0, stream, a);
+    // a workgroup for every rank while that makes some thousands; of many adapters most have no parts
+    const uint32_t across = std::min<uint32_t>((std::max(a.of[0].cols, a.of[1].cols) + 2047) / 2048, 64);
+    a.join = std::min(a.rank, std::max<uint32_t>(1, 4096 / a.g.adapters / across));
+    return launch_kernel(adapter_grad_join_kernel, dim3(a.g.adapters * a.join, across, 2), dim3(256), 0, stream, a);
 }
 
 }  // namespace qgemm

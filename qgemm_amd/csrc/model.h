@@ -120,11 +120,11 @@ struct AdapterGradArgs {
     RowGroups g;
     AdapterGrad of[2];
     const float *scaling;
-    uint32_t rank, chunk, tiles;         // tiles: column tiles of the first factor
+    uint32_t rank, chunk, tiles, join;   // tiles: column tiles of the first factor; join: workgroups that share an adapter's ranks out when parts are added up
     int dt, dw_dt;
 };
 size_t plan_adapter_grad(AdapterGradArgs &a, int cus);    // chooses chunk; bytes of both rooms, one behind the other
 void place_adapter_grad(AdapterGradArgs &a, float *room);
-hipError_t launch_adapter_grad(const AdapterGradArgs &a, hipStream_t stream);
+hipError_t launch_adapter_grad(AdapterGradArgs a, hipStream_t stream);
 
 }  // namespace qgemm
