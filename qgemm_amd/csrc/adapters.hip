@@ -19,12 +19,12 @@ auto with_ranks(uint32_t rank, F f) {
     if (rank <= 64) return f(std::integral_constant<int, 4>{});
     return f(std::integral_constant<int, 8>{});
 }
-// Slots that there are likely to be, by which work is shared out: of a few rows any may have an adapter of its own, many are prompts, and of the adapters
-// that there is room for most have no row.  (8192 rows of 32 prompts, 4096 x 4096 at rank 16, 1000 adapters, us: shrink and expand by the slots that there could be
-// 45 and 138, by these 27 and 75.)
+// Slots that there are likely to be, by which work is shared out.  Up to 1024 rows may be a decoding step whose requests all have adapters of their own; more are prompts, and of
+// the adapters that there is room for most then have no row.  (Rank 16, bf16, us of shrink + expand by the slots that there could be / by those of prompts: 512 rows of 500
+// adapters, 4096 x 4096 14 + 20 / 20 + 30; 1024 of 1000, 2048 x 8192 16 + 85 / 25 + 95; but 8192 rows of 32 prompts among 1000 adapters, 4096 x 4096 45 + 138 / 27 + 75.)
 uint32_t likely_slots(const RowGroups &g) {
-    const uint32_t whole = g.rows / kSlotRows;
-    return std::max<uint32_t>(1, std::min(g.slot_count, whole + std::min(g.adapters + 1, std::max<uint32_t>(64, whole))));
+    const uint32_t whole = g.rows / kSlotRows, groups = g.rows <= 1024 ? g.rows : std::max<uint32_t>(64, whole);
+    return std::max<uint32_t>(1, std::min(g.slot_count, whole + std::min(g.adapters + 1, groups)));
 }
 uint32_t column_tiles(uint32_t cols) { return (cols + 255) / 256; }
 }  // namespace
