@@ -275,6 +275,7 @@ int qgemm_add_adapters_backward(int dtype, int dx_dtype, int grad_dtype, const v
  * values log p, indices, equal ones in the order of their columns.
  *   tokens    rows integers of token_bytes 4 or 8; one outside 0 .. cols - 1 asks for nothing, and its logp is 0
  *   top       0 .. 32, at most cols; values and indices [rows x top]
+ * logp and values are (x - max x) - log S, S = sum exp(x - max x), and as exact in rows far from zero as in others; lse = max x + log S has there lost bits of log S.
  * -infinity is a column that cannot be.  A row of nothing else has lse = logp = -infinity and entropy 0; one with an infinity or a NaN gives NaNs
  * (its indices are those of its numbers, NaN counting as -infinity).  Uses the library workspace where rows are few. */
 int qgemm_log_probabilities(int dtype, int token_bytes, const void *logits, size_t ld, const void *tokens, int top, float *logp, float *entropy,

@@ -1,5 +1,6 @@
 // Log probabilities of given tokens out of logits, row by row: with m = max x, e = exp(x - m), S = sum e, T = sum e (x - m),
-//   lse = m + log S,   log p of a token = x[token] - lse,   entropy = log S - T / S,   and the largest x with x - lse;
+//   lse = m + log S,   log p of a token = (x[token] - m) - log S,   entropy = log S - T / S,   and the largest x with their log p;
+// (lse has lost bits of log S where m is far from zero, all of them in a row that is masked throughout with the type's lowest value)
 // and backward, with p = exp(x - lse), a = dlogp, b = dentropy:
 //   dx_j = a ([j = token] - p_j) - b p_j (log p_j + entropy).
 // One pass: every thread keeps the maximum of what it has seen, S and T under it, and puts them right when the maximum grows.  All fp32.
@@ -109,15 +110,15 @@ struct Asked {
     }
 };
 // a row's numbers out of its sums
-__device__ __forceinline__ void log_prob_finish(const LogProbArgs &p, uint32_t row, const Asked &asked, float s, float t, float l, float lse) {
+__device__ __forceinline__ void log_prob_finish(const LogProbArgs &p, uint32_t row, const Asked &asked, float m, float s, float t, float l) {
     const bool none = s == 0.0f;
-    p.logp[row] = !asked.any ? 0.0f : none ? kMinusInf : asked.logit - lse;
+    p.logp[row] = !asked.any ? 0.0f : none ? kMinusInf : (asked.logit - m) - l;
     p.entropy[row] = none ? 0.0f : l - t / s;
-    p.lse[row] = lse;
+    p.lse[row] = none ? kMinusInf : m + l;
 }
-__device__ __forceinline__ void store_top(const LogProbArgs &p, uint32_t row, uint32_t place, uint64_t key, float lse) {
+__device__ __forceinline__ void store_top(const LogProbArgs &p, uint32_t row, uint32_t place, uint64_t key, float m, float l) {
     const float v = value_of(key);
-    p.values[(size_t)row * p.top + place] = v == kMinusInf && lse == lse ? v : v - lse;
+    p.values[(size_t)row * p.top + place] = v == kMinusInf && l == l ? v : (v - m) - l;
     p.indices[(size_t)row * p.top + place] = index_of(key);
 }
 
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(kLogProbThreads) log_prob_kernel(const LogProb
             all_s += red[1][i];
             all_t += red[2][i];
         }
-        const float l = logf(all_s), lse = all_s == 0.0f ? kMinusInf : m + l;
+        const float l = logf(all_s);
         float *part = p.splits > 1 ? p.partial + ((size_t)row * p.splits + blockIdx.x) * log_prob_part(p.top) : nullptr;
         if (tid == 0) {
             if (part) {
@@ -268,14 +269,14 @@ __global__ void __launch_bounds__(kLogProbThreads) log_prob_kernel(const LogProb
                 part[1] = all_s;
                 part[2] = all_t;
             } else {
-                log_prob_finish(p, row, asked, all_s, all_t, l, lse);
+                log_prob_finish(p, row, asked, m, all_s, all_t, l);
             }
         }
         if constexpr (TOP) {
             const uint64_t own = begin + tid * kOctet < end ? key_of(best, best_at) : 0;
             top_of<DT>(x, begin, end, p.top, own, [&](uint32_t place, uint64_t key) {
                 if (part) ((uint64_t *)(part + 4))[place] = key;
-                else store_top(p, row, place, key, lse);
+                else store_top(p, row, place, key, m, l);
             });
         }
         __syncthreads();
@@ -305,8 +306,8 @@ __global__ void __launch_bounds__(256) log_prob_join_kernel(const LogProbArgs p)
         Sums sums{in ? part[0] : kMinusInf, in ? part[1] : 0.0f, in ? part[2] : 0.0f};
         const float m = wave_max(sums.m);
         sums.raise(m);
-        const float s = lanes_sum<64>(sums.s), t = lanes_sum<64>(sums.t), l = logf(s), lse = s == 0.0f ? kMinusInf : m + l;
-        if (tid == 0) log_prob_finish(p, row, asked, s, t, l, lse);
+        const float s = lanes_sum<64>(sums.s), t = lanes_sum<64>(sums.t), l = logf(s);
+        if (tid == 0) log_prob_finish(p, row, asked, m, s, t, l);
         if (!p.top) continue;
         if (place == 0) {
             bound = kth_largest(in ? bound : 0, p.top);
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(256) log_prob_join_kernel(const LogProbArgs p)
         for (uint32_t i = tid; i < found; i += 256) {
             const uint64_t mine = list[i];
             const uint32_t above = keys_above(list, found, mine);
-            if (above < p.top) store_top(p, row, above, mine, lse);
+            if (above < p.top) store_top(p, row, above, mine, m, l);
         }
         __syncthreads();
     }
