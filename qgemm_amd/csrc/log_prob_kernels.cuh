@@ -1,7 +1,7 @@
 // Log probabilities of given tokens out of logits, row by row: with m = max x, e = exp(x - m), S = sum e, T = sum e (x - m),
 //   lse = m + log S,   log p of a token = (x[token] - m) - log S,   entropy = log S - T / S,   and the largest x with their log p;
 // (lse has lost bits of log S where m is far from zero, all of them in a row that is masked throughout with the type's lowest value)
-// and backward, with p = exp(x - lse), a = dlogp, b = dentropy:
+// and backward, with p = exp(log p), a = dlogp, b = dentropy:
 //   dx_j = a ([j = token] - p_j) - b p_j (log p_j + entropy).
 // One pass: every thread keeps the maximum of what it has seen, S and T under it, and puts them right when the maximum grows.  All fp32.
 //
@@ -15,7 +15,7 @@
 //
 // What bounds it: memory, with the vector instructions (eleven slots an element, four of them the exponential) close behind: 2048 x 65536 bf16 with five tokens 61 us in a
 // trace, 4.4 TB/s; a plain sum of as many bytes reads 4.0.  8 x 131072 fp32 with twenty tokens 7.3 and 5 for the join, trips to memory and to LDS one behind
-// the other; backward 2048 x 65536 bf16 92, 5.9 TB/s read and written.
+// the other; backward 2048 x 65536 bf16 92, 5.8 TB/s read and written.
 #pragma once
 #include "model.h"
 #include "octet.cuh"
@@ -208,68 +208,78 @@ __device__ __forceinline__ void top_of(const void *row, uint32_t begin, uint32_t
     }
 }
 
+// A workgroup's sums of columns begin .. end - 1 of a row, in every thread; `each` is told of each octet's largest element and first column
+template <int DT, int AHEAD, class Each>
+__device__ __forceinline__ Sums row_sums(const char *x, uint32_t begin, uint32_t end, Each each) {
+    constexpr int WAVES = kLogProbThreads / 64;
+    __shared__ float red[3][WAVES];
+    const uint32_t tid = threadIdx.x;
+    Sums sums{kMinusInf, 0.0f, 0.0f};
+    for (uint32_t c0 = begin + tid * kOctet; c0 < end; c0 += AHEAD * kLogProbTurn) {
+        Octet<DT> o[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) o[i].request(x, c0 + i * kLogProbTurn, end);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const uint32_t c = c0 + i * kLogProbTurn;
+            if (c >= end) break;
+            float v[8];
+            o[i].settle(c, end);
+            o[i].floats(v);
+            if (end - c < kOctet)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = c + e < end ? v[e] : kMinusInf;
+            const float most = max8(v);
+            each(most, c);
+            sums.add(v, most);
+        }
+    }
+    const float wave = wave_max(sums.m);
+    if ((tid & 63) == 0) red[0][tid >> 6] = wave;
+    __syncthreads();
+    float m = red[0][0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) m = __builtin_fmaxf(m, red[0][i]);
+    sums.raise(m);
+    const float s = lanes_sum<64>(sums.s), t = lanes_sum<64>(sums.t);
+    if ((tid & 63) == 0) {
+        red[1][tid >> 6] = s;
+        red[2][tid >> 6] = t;
+    }
+    __syncthreads();                                       // (the next row's maxima go where nobody reads any more)
+    Sums all{m, red[1][0], red[2][0]};
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) {
+        all.s += red[1][i];
+        all.t += red[2][i];
+    }
+    return all;
+}
+
 // one workgroup for a split of a row
 template <int DT, bool TOP>
 __global__ void __launch_bounds__(kLogProbThreads) log_prob_kernel(const LogProbArgs p) {
-    constexpr int AHEAD = kLogProbAhead, WAVES = kLogProbThreads / 64;
-    __shared__ float red[3][WAVES];
     const uint32_t tid = threadIdx.x, begin = blockIdx.x * p.part, end = p.cols - begin < p.part ? p.cols : begin + p.part;
     for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
         const char *x = (const char *)p.logits + (size_t)row * p.ld * Octet<DT>::ES;
         const Asked asked(p, row);
-        Sums sums{kMinusInf, 0.0f, 0.0f};
         float best = kMinusInf;
         uint32_t best_at = begin + tid * kOctet;
-        for (uint32_t c0 = begin + tid * kOctet; c0 < end; c0 += AHEAD * kLogProbTurn) {
-            Octet<DT> o[AHEAD];
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) o[i].request(x, c0 + i * kLogProbTurn, end);
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                const uint32_t c = c0 + i * kLogProbTurn;
-                if (c >= end) break;
-                float v[8];
-                o[i].settle(c, end);
-                o[i].floats(v);
-                if (end - c < kOctet)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = c + e < end ? v[e] : kMinusInf;
-                const float most = max8(v);
-                if (TOP && most > best) {
-                    best = most;
-                    best_at = c;
-                }
-                sums.add(v, most);
+        const Sums sums = row_sums<DT, kLogProbAhead>(x, begin, end, [&](float most, uint32_t c) {
+            if (TOP && most > best) {
+                best = most;
+                best_at = c;
             }
-        }
-        const float wave = wave_max(sums.m);
-        if ((tid & 63) == 0) red[0][tid >> 6] = wave;
-        __syncthreads();
-        float m = red[0][0];
-#pragma unroll
-        for (int i = 1; i < WAVES; ++i) m = __builtin_fmaxf(m, red[0][i]);
-        sums.raise(m);
-        const float s = lanes_sum<64>(sums.s), t = lanes_sum<64>(sums.t);
-        if ((tid & 63) == 0) {
-            red[1][tid >> 6] = s;
-            red[2][tid >> 6] = t;
-        }
-        __syncthreads();
-        float all_s = red[1][0], all_t = red[2][0];
-#pragma unroll
-        for (int i = 1; i < WAVES; ++i) {
-            all_s += red[1][i];
-            all_t += red[2][i];
-        }
-        const float l = logf(all_s);
+        });
+        const float m = sums.m, l = logf(sums.s);
         float *part = p.splits > 1 ? p.partial + ((size_t)row * p.splits + blockIdx.x) * log_prob_part(p.top) : nullptr;
         if (tid == 0) {
             if (part) {
                 part[0] = m;
-                part[1] = all_s;
-                part[2] = all_t;
+                part[1] = sums.s;
+                part[2] = sums.t;
             } else {
-                log_prob_finish(p, row, asked, m, all_s, all_t, l);
+                log_prob_finish(p, row, asked, m, sums.s, sums.t, l);
             }
         }
         if constexpr (TOP) {
@@ -337,7 +347,11 @@ __global__ void __launch_bounds__(256) log_prob_join_kernel(const LogProbArgs p)
     }
 }
 
-// ---- backward: a workgroup takes AHEAD times kLogProbTurn columns a turn
+// ---- backward: a workgroup takes AHEAD times kLogProbTurn columns a turn.  log p = x - lse is off by the rounding of lse, half its last place: 2^-18 of p at kFar, as much as
+// the exponential's own roundings leave of p = exp(-30).  Beyond it, up to where lse holds nothing of log S, one workgroup sums the row again and writes all of it with
+// log p = (x - m) - log S.  (us, no row / every row beyond: 2048 x 65536 bf16 112 / 230, fp32 183 / 400, 8 x 131072 fp32 4 / 52.  The choice costs rows that are near
+// 1.4 us of 2048 x 65536: 90.9 without it, 92.3 so, 94.5 with what the row asks for fetched one behind the other.)
+constexpr float kFar = 128.0f;
 template <int DT>
 __global__ void __launch_bounds__(kLogProbThreads) log_prob_backward_kernel(const LogProbBackwardArgs p) {
     constexpr uint32_t AHEAD = 2;
@@ -346,13 +360,26 @@ __global__ void __launch_bounds__(kLogProbThreads) log_prob_backward_kernel(cons
         char *dx = (char *)p.dlogits + (size_t)row * p.ldd * dtype_bytes(p.out_dt);
         const int64_t token = token_at(p.tokens, p.token_bytes, row);
         const bool asked = token >= 0 && token < (int64_t)p.cols;
-        const float lse = p.lse[row], b = p.dentropy ? p.dentropy[row] : 0.0f, h = b != 0.0f ? p.entropy[row] : 0.0f;
-        const bool none = lse == kMinusInf;
-        const float a = asked && !none ? p.dlogp[row] : 0.0f;
-        for (uint32_t c0 = blockIdx.x * AHEAD * kLogProbTurn + threadIdx.x * kOctet; c0 < p.cols; c0 += gridDim.x * AHEAD * kLogProbTurn) {
-            Octet<DT> o[AHEAD];
+        const float lse = p.lse[row], dlogp = p.dlogp[row], b = p.dentropy ? p.dentropy[row] : 0.0f, entropy = p.dentropy ? p.entropy[row] : 0.0f;
+        const bool none = lse == kMinusInf, far = __builtin_fabsf(lse) > kFar && __builtin_fabsf(lse) < __builtin_inff();
+        const float a = asked && !none ? dlogp : 0.0f, h = b != 0.0f ? entropy : 0.0f;      // (chosen when they are there: no trip to memory behind another)
+        Octet<DT> o[AHEAD];
+        auto request = [&](uint32_t c0) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) o[i].request(x, c0 + i * kLogProbTurn, p.cols);
+        };
+        constexpr uint32_t turn = AHEAD * kLogProbTurn;
+        uint32_t c0 = blockIdx.x * turn + threadIdx.x * kOctet, step = gridDim.x * turn;
+        float m = lse, log_s = 0.0f;
+        request(c0);
+        if (far) {
+            if (blockIdx.x != row % gridDim.x) continue;       // (the first of each row would be on the same XCD where their number is a multiple of 8)
+            const Sums sums = row_sums<DT, AHEAD>(x, 0, p.cols, [](float, uint32_t) {});
+            c0 = threadIdx.x * kOctet, step = turn;
+            m = sums.m, log_s = logf(sums.s);
+            request(c0);
+        }
+        for (; c0 < p.cols; c0 += step) {
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
                 const uint32_t c = c0 + i * kLogProbTurn;
@@ -362,7 +389,7 @@ __global__ void __launch_bounds__(kLogProbThreads) log_prob_backward_kernel(cons
                 o[i].floats(v);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float l = v[e] - lse, q = none ? 0.0f : exp_of(l);
+                    const float l = (v[e] - m) - log_s, q = none ? 0.0f : exp_of(l);
                     const float g = a + b * (__builtin_fmaxf(l, kNothing) + h);
                     v[e] = -(q * g);
                     if (asked && (int64_t)(c + e) == token) v[e] += a;
@@ -372,6 +399,7 @@ __global__ void __launch_bounds__(kLogProbThreads) log_prob_backward_kernel(cons
                     for (int e = 0; e < 8; ++e) v[e] = 0.0f;
                 store_octet(dx, p.out_dt, c, p.cols, v);
             }
+            if (p.cols - c0 > step) request(c0 + step);
         }
     }
 }
