@@ -284,7 +284,8 @@ int qgemm_log_probabilities(int dtype, int token_bytes, const void *logits, size
 /* Backward pass: dlogits_j = dlogp * ([j = token] - p_j) - dentropy * p_j * (log p_j + entropy), of out_dtype
  *   lse, entropy  as qgemm_log_probabilities gave them; dentropy NULL: zeros (entropy may be NULL then)
  * p = exp(x - lse) where |lse| is up to 128; in rows farther from zero lse has lost more of log sum exp than that leaves, and the row is summed again.
- * A row of nothing but -infinity has the gradient 0, and so has the logp of a row whose token asks for nothing. */
+ * A row of nothing but -infinity has the gradient 0, and so has the logp of a row whose token asks for nothing: with dentropy 0 such a row's gradient
+ * is 0 whatever it holds, NaN too. */
 int qgemm_log_probabilities_backward(int dtype, int out_dtype, int token_bytes, const void *logits, size_t ld, const void *tokens, const float *lse,
                                      const float *entropy, const float *dlogp, const float *dentropy, void *dlogits, size_t ldd, size_t rows,
                                      size_t cols, void *stream);

@@ -363,6 +363,7 @@ __global__ void __launch_bounds__(kLogProbThreads) log_prob_backward_kernel(cons
         const float lse = p.lse[row], dlogp = p.dlogp[row], b = p.dentropy ? p.dentropy[row] : 0.0f, entropy = p.dentropy ? p.entropy[row] : 0.0f;
         const bool none = lse == kMinusInf, far = __builtin_fabsf(lse) > kFar && __builtin_fabsf(lse) < __builtin_inff();
         const float a = asked && !none ? dlogp : 0.0f, h = b != 0.0f ? entropy : 0.0f;      // (chosen when they are there: no trip to memory behind another)
+        const bool nothing = !asked && b == 0.0f;      // (padding may hold anything: 0 times its NaNs is no 0)
         Octet<DT> o[AHEAD];
         auto request = [&](uint32_t c0) __attribute__((always_inline)) {
 #pragma unroll
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(kLogProbThreads) log_prob_backward_kernel(cons
                     v[e] = -(q * g);
                     if (asked && (int64_t)(c + e) == token) v[e] += a;
                 }
-                if (none)
+                if (none || nothing)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] = 0.0f;
                 store_octet(dx, p.out_dt, c, p.cols, v);

@@ -160,3 +160,23 @@ def test_gradients_far_from_zero_in_a_graph():
         torch.cuda.synchronize()
         got = [t.clone() for t in out]
         assert all(torch.equal(p, q) for p, q in zip(got, both()))
+
+
+@pytest.mark.parametrize("cols", [30, 5000])
+@pytest.mark.parametrize("bonus", [None, 0.0, 1.0])
+def test_padding_rows_have_no_gradient_whatever_they_hold(cols, bonus):
+    """Rows that ask for nothing, with NaN and infinities in them: no gradient comes of their log p, and none of an entropy that has no gradient."""
+    say("log_probabilities_backward padding", cols, bonus)
+    x, tokens = torch.randn(6, cols, generator=torch.Generator().manual_seed(1)).cuda(), torch.tensor([3, -100, -100, cols, 4, -100], device="cuda")
+    x[1], x[2, 5], x[3, 0] = float("nan"), float("inf"), float("nan")
+    _, entropy, lse = Q.log_probabilities(x, tokens)
+    a, b = torch.ones(6, device="cuda"), None if bonus is None else torch.zeros(6, device="cuda")
+    a[3] = float("nan")
+    if bonus:
+        b[0], b[5] = bonus, bonus
+    dx = Q.log_probabilities_backward(x, tokens, lse, entropy if bonus is not None else None, a, b)
+    assert (dx[1:4] == 0).all() and torch.isfinite(dx).all()
+    assert ((dx[5] != 0).any() if bonus else (dx[5] == 0).all()) and (dx[0] != 0).any() and (dx[4] != 0).any()
+    if bonus:
+        b[1] = bonus                                       # (an entropy that is asked for is NaN, and so is its gradient)
+        assert torch.isnan(Q.log_probabilities_backward(x, tokens, lse, entropy, a, b)[1]).all()
