@@ -277,7 +277,8 @@ int qgemm_add_adapters_backward(int dtype, int dx_dtype, int grad_dtype, const v
  *   top       0 .. 32, at most cols; values and indices [rows x top]
  * logp and values are (x - max x) - log S, S = sum exp(x - max x), and as exact in rows far from zero as in others; lse = max x + log S has there lost bits of log S.
  * -infinity is a column that cannot be.  A row of nothing else has lse = logp = -infinity and entropy 0; one with an infinity or a NaN gives NaNs
- * (its indices are those of its numbers, NaN counting as -infinity).  Uses the library workspace where rows are few. */
+ * (its indices are those of its numbers, NaN counting as -infinity).  Uses the library workspace where rows are few: long rows are split then, and the last bits of
+ * logp, entropy, lse and values may depend on how many rows there are (the indices do not). */
 int qgemm_log_probabilities(int dtype, int token_bytes, const void *logits, size_t ld, const void *tokens, int top, float *logp, float *entropy,
                             float *lse, float *values, int64_t *indices, size_t rows, size_t cols, void *stream);
 
