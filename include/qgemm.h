@@ -256,7 +256,9 @@ int qgemm_group_rows(int id_bytes, const void *ids, size_t rows, size_t adapters
  *   scaling   adapters floats, or NULL: 1
  *   groups    of these rows and this number of adapters
  *   u         A[i] x[t] for the backward pass, rows x rank floats (zeros for rows of no adapter), or NULL
- * A[i] x[t] has fp32 accumulators and goes on in 16 bits of mantissa, in 24 where y is F32.  Uses the library workspace.  Up to 2^23 - 256 columns. */
+ * A[i] x[t] has fp32 accumulators and goes on in 16 bits of mantissa, in 24 where y is F32.  Uses the library workspace.  Up to 2^23 - 256 columns.
+ * An infinity in A, B or x makes infinities or NaNs of the results that depend on it, NaN also where the formula gives an infinity, and of no others; so here and in the
+ * backward pass (dy as well). */
 int qgemm_add_adapters(int dtype, int y_dtype, const void *y, size_t ldy, const void *x, size_t ldx, const void *A, const void *B,
                        const float *scaling, const void *groups, void *out, size_t ldo, float *u, size_t rows, size_t adapters,
                        size_t rank, size_t k, size_t n, void *stream);

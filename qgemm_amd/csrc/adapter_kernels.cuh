@@ -9,7 +9,8 @@
 //
 // u and v are fp32.  Where they are an operand of the matrix cores they are split into bf16 numbers that add up to them, two of them (16 bits) where
 // the result has 16 bits, three (24) where it has 32; fp16 operands beside them are split into two, exactly, which keeps bf16's exponents:
-// gradients are often below what fp16 holds.
+// gradients are often below what fp16 holds.  An infinite operand meets all parts of the other, of which some are 0 or have the other sign: what depends on it is
+// infinite or NaN, not always the formula's infinity.  (The sums of a result are its own: nothing else changes.)
 //
 // What bounds them, times of the kernels in a trace: memory, and for few rows the chain of trips to it (slot, order, operands) behind a launch.  64 rows of 48 adapters of
 // rank 16, 4096 x 4096: group 2.8 us, shrink 4.4, expand 6.4; 8192 rows of 8 adapters of rank 32: 6.2, 16.6 and 31.2 (4.0 TB/s of x; 4.3 of y in and out).  Backward of 4096 rows of
