@@ -6,7 +6,7 @@
 namespace qgemm {
 
 namespace {
-constexpr size_t kMostRoom = (size_t)128 << 20;       // partial sums that a stream's own workspace block holds
+constexpr size_t kMostRoom = (size_t)128 << 20;       // the gradients' partial sums (sums over the rank lie in front of them: together they may pass a stream's own workspace block)
 
 template <class F>
 auto with_dt(int dt, F f) {
