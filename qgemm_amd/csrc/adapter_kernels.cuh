@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(256, (expand_waves<DT, Y_DT, RANKS, ROW>())) a
     request_y(from);
     const float by = plain || !p.scaling ? 1.0f : p.scaling[s.adapter];
     // the rank's sums of the slot's rows, in parts: a lane has EACH quads of them (what lies behind the rows goes into products that nobody stores)
-    constexpr int EACH = (int)kSlotRows * QUADS / 256, BATCH = 1;
+    constexpr int EACH = (int)kSlotRows * QUADS / 256;
     uint32_t sum_row[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
@@ -429,37 +429,28 @@ __global__ void __launch_bounds__(256, (expand_waves<DT, Y_DT, RANKS, ROW>())) a
         sum_row[i] = sums_row(p.u, p.g, s.begin + (at < s.count ? at : s.count - 1));
     }
 #pragma unroll
-    for (int i0 = 0; i0 < EACH; i0 += BATCH) {
-        if (256 * i0 / QUADS >= (int)s.count) break;
-        v4f sum[BATCH];
+    for (int i = 0; i < EACH; ++i) {
+        if (256 * i / QUADS >= (int)s.count) break;
+        const uint32_t n = tid + 256 * i, at = n / QUADS, q = n % QUADS * 4;
+        v4f v = q < ranks ? rank_sums(p.u, sum_row[i], q, ranks) : v4f{};
+        if (at >= s.count) break;
+        if (p.keep && blockIdx.y == 0) {
+            const size_t to_row = p.keep_grouped ? s.begin + at : (uint32_t)p.g.order[s.begin + at];
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const uint32_t q = (tid + 256 * (i0 + i)) % QUADS * 4;
-            sum[i] = q < ranks ? rank_sums(p.u, sum_row[i0 + i], q, ranks) : v4f{};
+            for (uint32_t e = 0; e < 4; ++e)
+                if (q + e < p.rank) p.keep[to_row * p.rank + q + e] = v[e];
         }
+        v *= by;
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const uint32_t n = tid + 256 * (i0 + i), at = n / QUADS, q = n % QUADS * 4;
-            if (at >= s.count) break;
-            v4f v = sum[i];
-            if (p.keep && blockIdx.y == 0) {
-                const size_t to_row = p.keep_grouped ? s.begin + at : (uint32_t)p.g.order[s.begin + at];
+        for (int part = 0; part < PARTS; ++part) {
+            uint32_t h[4];
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e)
-                    if (q + e < p.rank) p.keep[to_row * p.rank + q + e] = v[e];
+            for (int e = 0; e < 4; ++e) {
+                float x = v[e];
+                h[e] = split_off(x);
+                v[e] = x;
             }
-            v *= by;
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part) {
-                uint32_t h[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = v[e];
-                    h[e] = split_off(x);
-                    v[e] = x;
-                }
-                *(v2i *)(sums[part] + at * PITCH + q * 2) = v2i{(int)(h[0] | h[1] << 16), (int)(h[2] | h[3] << 16)};
-            }
+            *(v2i *)(sums[part] + at * PITCH + q * 2) = v2i{(int)(h[0] | h[1] << 16), (int)(h[2] | h[3] << 16)};
         }
     }
     if (plain && (const void *)p.out == p.y) return;

@@ -13,7 +13,7 @@ struct RmsArgs {
     float eps;
     int x_dt, r_dt, y_dt, param_dt, q_dt;
 };
-hipError_t launch_rms_norm(const RmsArgs &a, int cus, hipStream_t stream);
+hipError_t launch_rms_norm(const RmsArgs &a, hipStream_t stream);
 
 struct RmsBackwardArgs {
     const void *dy, *h, *dh, *weight;    // dh: what arrives along the residual stream, or null

@@ -2266,7 +2266,7 @@ QGEMM_EXPORT int qgemm_rms_norm(int x_dtype, int residual_dtype, int y_dtype, in
     a.eps = eps;
     a.x_dt = x_dtype, a.r_dt = residual ? residual_dtype : x_dtype, a.y_dt = y_dtype, a.param_dt = param_dtype, a.q_dt = q_dtype;
     g_ctx.last_config = "rms_norm";
-    return launch_rms_norm(a, g_ctx.num_cus, (hipStream_t)stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
+    return launch_rms_norm(a, (hipStream_t)stream) == hipSuccess ? QGEMM_OK : QGEMM_ERR_LAUNCH;
 }
 
 QGEMM_EXPORT int qgemm_rms_norm_backward(int dy_dtype, int h_dtype, int dh_dtype, int dx_dtype, int param_dtype, const void *dy, size_t lddy, const void *h,

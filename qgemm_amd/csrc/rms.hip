@@ -78,7 +78,7 @@ auto with_type(int dt, F f) {
 }
 }  // namespace
 
-hipError_t launch_rms_norm(const RmsArgs &a, int, hipStream_t stream) {
+hipError_t launch_rms_norm(const RmsArgs &a, hipStream_t stream) {
     if (in_registers(a.cols) && (!a.residual || a.r_dt == a.x_dt || a.r_dt == QGEMM_DT_F32))
         return with_shape(forward_shape(a.cols), [&](auto group, auto p) {
             return with_type(a.x_dt, [&](auto dt) {
