@@ -410,6 +410,13 @@ std::tuple<int, at::Tensor> ops_group_rows(const at::Tensor &ids, int64_t adapte
     return {qgemm_group_rows(bytes, ids.data_ptr(), ids.numel(), adapters, out.data_ptr(), current_stream()), out};
 }
 
+// what group_rows() gives for these numbers, by its size (its contents are not looked at)
+bool groups_ok(const at::Tensor &words, int64_t rows, int64_t adapters) {
+    size_t n;
+    return rows >= 0 && adapters > 0 && qgemm_group_rows_words(rows, adapters, &n) == QGEMM_OK && here(words) && words.scalar_type() == at::kInt && words.is_contiguous() &&
+           words.numel() == (int64_t)n;
+}
+
 // a factor of the adapters, [adapters][rank][cols]
 bool factor_ok(const at::Tensor &w, const at::Tensor &x, int64_t adapters, int64_t &rank, int64_t &cols) {
     if (!here(w) || w.scalar_type() != x.scalar_type() || w.dim() != 3 || !w.is_contiguous() || w.size(0) != adapters) return false;
@@ -425,7 +432,7 @@ std::tuple<int, at::Tensor, at::Tensor> ops_add_adapters(const at::Tensor &y, co
     const std::tuple<int, at::Tensor, at::Tensor> not_plain{kNotPlain, at::Tensor(), at::Tensor()};
     int64_t xrows, k, ldx, rank, rank_b, ka, n, ldy, ldo;
     const int dt = plain_dtype(x, false), ydt = plain_dtype(y, false);
-    if ((dt != QGEMM_DT_BF16 && dt != QGEMM_DT_F16) || !float_dtype(ydt) || !here(x) || !here(words) || !here(scaling) || !rows_of(x, xrows, k, ldx) || xrows != rows ||
+    if ((dt != QGEMM_DT_BF16 && dt != QGEMM_DT_F16) || !float_dtype(ydt) || !here(x) || !groups_ok(words, rows, adapters) || !here(scaling) || !rows_of(x, xrows, k, ldx) || xrows != rows ||
         !factor_ok(A, x, adapters, rank, ka) || !factor_ok(B, x, adapters, rank_b, n) || ka != k || rank_b != rank || !rows_like(y, rows, n, ldy) ||
         (scaling && !float_vector(*scaling, adapters)))
         return not_plain;
@@ -446,7 +453,7 @@ std::tuple<int, at::Tensor, at::Tensor, at::Tensor> ops_add_adapters_backward(co
     const std::tuple<int, at::Tensor, at::Tensor, at::Tensor> not_plain{kNotPlain, at::Tensor(), at::Tensor(), at::Tensor()};
     int64_t xrows, k, ldx, rank, rank_b, ka, n, lddy, ld0 = 0;
     const int dt = plain_dtype(x, false), dxdt = dx0 ? plain_dtype(*dx0, false) : dt;
-    if ((dt != QGEMM_DT_BF16 && dt != QGEMM_DT_F16) || !float_dtype(dxdt) || !here(x) || !here(u) || !here(words) || !here(scaling) || !rows_of(x, xrows, k, ldx) ||
+    if ((dt != QGEMM_DT_BF16 && dt != QGEMM_DT_F16) || !float_dtype(dxdt) || !here(x) || !here(u) || !groups_ok(words, rows, adapters) || !here(scaling) || !rows_of(x, xrows, k, ldx) ||
         xrows != rows || !factor_ok(A, x, adapters, rank, ka) || !factor_ok(B, x, adapters, rank_b, n) || ka != k || rank_b != rank ||
         dy.scalar_type() != x.scalar_type() || !rows_like(dy, rows, n, lddy) || !float_vector(u, rows * rank) || (dx0 && !rows_like(*dx0, rows, k, ld0)) ||
         (scaling && !float_vector(*scaling, adapters)) || (grad != at::kFloat && grad != at::kBFloat16 && grad != at::kHalf))

@@ -606,6 +606,11 @@ def _adapters(x, A, B, groups, scaling):
     if not isinstance(groups, RowGroups):
         raise TypeError(f"groups must be what group_rows() gives, got {type(groups).__name__}")
     _need_here(x, A, B, groups.words, scaling)
+    n = C.c_size_t()
+    check(load_library().qgemm_group_rows_words(groups.rows, groups.adapters, C.byref(n)))
+    _need_type(groups.words, (torch.int32,), "groups")
+    if groups.words.numel() != n.value or not groups.words.is_contiguous():
+        raise ValueError(f"groups must be what group_rows() gives for {groups.rows} rows and {groups.adapters} adapters")
     rows, k, ldx = _rows_of(x, "x")
     _need_type(x, _FLOATS[1:], "x")
     for t, name in ((A, "A"), (B, "B")):
