@@ -245,7 +245,7 @@ int qgemm_rms_norm_backward(int dy_dtype, int h_dtype, int dh_dtype, int dx_dtyp
 /* Rows grouped by the adapter that each of them has, once for all calls below with the same ids.
  *   ids      rows integers of id_bytes 4 or 8: 0 .. adapters - 1; any other number means no adapter
  *   groups   device memory of qgemm_group_rows_words 32-bit words, 16-byte aligned; its contents are the library's own
- * Up to 65535 adapters and 2^28 - 1 rows. */
+ * Up to 65535 adapters and 2^28 - 1 rows.  All ids are read for each adapter: about 1 us for a million of rows x adapters (65536 rows of 1000 adapters 78 us, 8192 of 65535 a millisecond). */
 int qgemm_group_rows_words(size_t rows, size_t adapters, size_t *words);
 int qgemm_group_rows(int id_bytes, const void *ids, size_t rows, size_t adapters, void *groups, void *stream);
 
